@@ -335,6 +335,56 @@ int32_t parpy_b200_viterbi_status(uint32_t *status);
  * without any kernel being starved. */
 int32_t parpy_b200_viterbi_wait_probe(int32_t polls, void *stream);
 
+/* ---- rows of vocabulary logits ------------------------------------------------------------
+ * No counterpart in the reference; its nearest function is test/test_softmax.py:11-26.
+ * x is [N, M] of element type `dtype`, its columns contiguous and its rows ldx elements
+ * apart (any pitch >= M and any alignment of the element type); z = x / temperature, with
+ * temperature in [1e-4, 1e4]. A logit of -inf is a column that a mask took out. Sums are kept in
+ * 32 bits, each output is rounded once. A row that holds a NaN or +inf gets NaN outputs
+ * (top_index -1); a row without a finite logit has lse -inf, logp -inf and a zero
+ * gradient. Token and column numbers are 64-bit where the wide_ flag is set, else 32-bit. */
+#define PARPY_B200_F32 0
+#define PARPY_B200_BF16 1
+#define PARPY_B200_F16 2
+
+/* For each row: lse[i] = log sum exp(z[i,:]); logp[i] = z[i, tokens[i]] - lse[i] (0 for a
+ * negative token, NaN for one >= M); entropy[i] = -sum p log p (0 without a finite logit);
+ * the K (0..128, <= M) largest logits as log-probabilities top_logp[N, K] and columns
+ * top_index[N, K], in falling order, ties by the lowest column. logp and tokens, entropy,
+ * and with K = 0 the alternatives may be NULL. */
+int32_t parpy_b200_token_logprobs(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                  const void *tokens, int32_t wide_tokens, double temperature, int64_t K,
+                                  float *logp, float *lse, float *entropy, float *top_logp, void *top_index,
+                                  int32_t wide_index, void *stream);
+/* Gradient with respect to x of sum(dlogp logp + dentropy entropy), from the lse and entropy that
+ * the call above wrote: dx[N, M] (rows lddx apart) of x's element type, which may be x itself.
+ * dlogp, dentropy (and then tokens, entropy) may be NULL: no such term. */
+int32_t parpy_b200_token_logprobs_grad(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                       const void *tokens, int32_t wide_tokens, double temperature,
+                                       const float *lse, const float *entropy, const float *dlogp,
+                                       const float *dentropy, void *dx, int64_t lddx, void *stream);
+
+/* Distance of the student's row from a teacher that is known by its K (1..1024) best columns:
+ * index[N, K], and values[N, K] (element type value_dtype), the teacher's logits or log-probabilities at
+ * the temperature wanted (what token_logprobs writes as top_logp; `temperature` scales the student).
+ * tail = 0: q = softmax of the listed values, loss = sum q (log q - log p).
+ * tail = 1: q = exp(values), and the mass 1 - sum q of all other columns against the student's
+ * there: + left (log left - (rest - lse)), rest = log sum exp(z) over the columns not listed.
+ * A negative index is an entry the teacher did not give; a column's second mention in a row is
+ * not used; an index >= M makes the row NaN. A row without an entry has loss 0 and no gradient.
+ * Writes loss[N], lse[N] and, with a tail, rest[N]. */
+int32_t parpy_b200_distill_topk(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                const void *index, int32_t wide_index, const void *values, int32_t value_dtype,
+                                int64_t K, double temperature, int32_t tail, float *loss, float *lse, float *rest,
+                                void *stream);
+/* Gradient with respect to x of sum(dloss loss), from the lse and rest that the call above
+ * wrote; dx as in token_logprobs_grad. */
+int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                     const void *index, int32_t wide_index, const void *values,
+                                     int32_t value_dtype, int64_t K, double temperature, int32_t tail,
+                                     const float *lse, const float *rest, const float *dloss, void *dx,
+                                     int64_t lddx, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,8 +68,14 @@ def _stage_one(arg, role, where, staged):
         return arg
     if isinstance(arg, Buffer):
         return arg
+    pitched = role.endswith("_rows")    # a CUDA array whose rows may lie apart
+    if pitched:
+        role = role[:-5]
+    import torch
+    if type(arg) is torch.Tensor and arg.is_cuda and arg.layout is torch.strided:
+        return CudaBuffer._from_array(arg, pitched)
     if hasattr(arg, "__cuda_array_interface__"):
-        return CudaBuffer._from_array(arg)
+        return CudaBuffer._from_array(arg, pitched)
     if hasattr(arg, "__array_interface__") or hasattr(arg, "__array__"):
         import torch
         from .buffer import _extract_array_interface, _host_view

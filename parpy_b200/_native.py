@@ -72,7 +72,19 @@ SIGNATURES = {
     "parpy_b200_viterbi_status": (c_i32, [c_ptr]),
     "parpy_b200_viterbi_wait_probe": (c_i32, [c_i32, c_ptr]),
     "parpy_b200_forward_wait_probe": (c_i32, [c_i32, c_ptr]),
+    "parpy_b200_token_logprobs": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_f64, c_i64, c_ptr,
+                                          c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr]),
+    "parpy_b200_token_logprobs_grad": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_f64, c_ptr, c_ptr,
+                                               c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
+    "parpy_b200_distill_topk": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_i64, c_f64,
+                                        c_i32, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "parpy_b200_distill_topk_grad": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_i64,
+                                             c_f64, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
 }
+
+# element types, and the most alternatives / list entries of a row, of the logits entries
+F32, BF16, F16 = 0, 1, 2
+TOP_MAX, LIST_MAX = 128, 1024
 
 REDUCE_SUM, REDUCE_PROD, REDUCE_MAX, REDUCE_MIN = 0, 1, 2, 3
 

@@ -8,9 +8,14 @@ from .options import CompileBackend
 backends = [CompileBackend.Cuda]
 
 
+_usable = set()   # (device, library) pairs that have passed the checks below
+
+
 def _assert_cuda_is_enabled():
     import torch
     from . import _native
+    if _usable and (torch.cuda.current_device(), _native.LIB_PATH) in _usable:
+        return
     if not torch.cuda.is_available():
         raise RuntimeError("No CUDA device is visible to torch")
     if not os.path.exists(_native.LIB_PATH):
@@ -18,6 +23,7 @@ def _assert_cuda_is_enabled():
     major, minor = torch.cuda.get_device_capability()
     if major < 10:
         raise RuntimeError(f"parpy_b200 kernels need compute capability 10.x, found {major}.{minor}")
+    _usable.add((torch.cuda.current_device(), _native.LIB_PATH))
 
 
 def is_enabled(backend, verbose=False):

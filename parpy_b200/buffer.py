@@ -20,7 +20,7 @@ import numpy as np
 from .options import CompileBackend, DataType, ElemSize
 
 
-def _check_array_interface(intf):
+def _check_array_interface(intf, pitched=False):
     shape = tuple(intf["shape"])
     dtype = DataType(intf["typestr"])
     if "data" in intf and intf["data"] is not None:
@@ -29,19 +29,29 @@ def _check_array_interface(intf):
             raise ValueError("Cannot construct buffer from read-only memory")
     else:
         raise ValueError("Buffer protocol not supported")
-    if intf.get("strides") is not None:
+    if intf.get("strides") is not None and not pitched:
         raise ValueError("Buffers must only operate on contiguous memory")
     return shape, dtype, data
 
 
-def _extract_array_interface(a, allow_cuda=False):
+def _extract_array_interface(a, allow_cuda=False, pitched=False):
     if allow_cuda and hasattr(a, "__cuda_array_interface__"):
-        return _check_array_interface(a.__cuda_array_interface__)
+        return _check_array_interface(a.__cuda_array_interface__, pitched)
+    if _is_host_bf16(a):
+        if not a.is_contiguous():
+            raise ValueError("Buffers must only operate on contiguous memory")
+        return tuple(a.shape), DataType("<V2"), a.data_ptr()
     if hasattr(a, "__array_interface__"):
         return _check_array_interface(a.__array_interface__)
     if hasattr(a, "__array__"):
         return _check_array_interface(a.__array__().__array_interface__)
     raise ValueError("Failed to extract array interface")
+
+
+def _is_host_bf16(a):
+    # NumPy has no bfloat16, so such a tensor has no array interface
+    import torch
+    return isinstance(a, torch.Tensor) and a.dtype == torch.bfloat16 and not a.is_cuda
 
 
 def _resolve_dtype(dtype):
@@ -71,6 +81,20 @@ def _host_view(t):
     if arr.dtype in (np.uint16, np.uint32, np.uint64):
         arr = arr.view({2: np.int16, 4: np.int32, 8: np.int64}[arr.dtype.itemsize])
     return torch.from_numpy(arr)
+
+
+_dtype_of = {}
+
+
+def _torch_dtypes():
+    """torch dtype -> DataType of its array interface."""
+    if not _dtype_of:
+        import torch
+        _dtype_of.update({getattr(torch, name): DataType(s) for name, s in (
+            ("bool", "|b1"), ("uint8", "|u1"), ("int8", "|i1"), ("int16", "<i2"), ("int32", "<i4"),
+            ("int64", "<i8"), ("float16", "<f2"), ("bfloat16", "<V2"), ("float32", "<f4"),
+            ("float64", "<f8"))})
+    return _dtype_of
 
 
 class Buffer:
@@ -121,7 +145,10 @@ class CudaBuffer(Buffer):
 
     def __init__(self, buf, shape, dtype, src=None, refcount=None):
         super().__init__(buf, shape, dtype, src, refcount)
-        self.__cuda_array_interface__ = buf.__cuda_array_interface__
+
+    @property
+    def __cuda_array_interface__(self):
+        return self.buf.__cuda_array_interface__
 
     def __del__(self):
         try:
@@ -144,10 +171,16 @@ class CudaBuffer(Buffer):
         self.src = None
 
     @staticmethod
-    def _from_array(t):
+    def _from_array(t, pitched=False):
+        """Wraps a CUDA array in place or copies a host array to the device. ``pitched``: the
+        operator takes the strides of a CUDA array, so that it need not be contiguous."""
         import torch
+        if type(t) is torch.Tensor and t.is_cuda and not t.requires_grad and t.layout is torch.strided:
+            dtype = _torch_dtypes().get(t.dtype)
+            if dtype is not None and (pitched or t.is_contiguous()):
+                return CudaBuffer(t, t.shape, dtype)    # what the array interface says, without building it
         try:
-            shape, dtype, _ = _extract_array_interface(t, allow_cuda=True)
+            shape, dtype, _ = _extract_array_interface(t, allow_cuda=True, pitched=pitched)
         except ValueError as e:
             raise ValueError(f"Cannot convert argument to a CUDA buffer: {e}")
         if hasattr(t, "__cuda_array_interface__"):

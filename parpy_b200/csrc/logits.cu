@@ -1,0 +1,1031 @@
+// Operators on rows of vocabulary logits for sm_100a: log-probabilities of given tokens with the row's entropy and
+// its K best alternatives, distillation from a teacher's K best logits, and both gradients.
+//
+// With z = x / temperature and a row's log-sum-exp lse = log sum_j exp(z_j), p_j = exp(z_j - lse):
+//
+//   token_logprobs   logp = z_t - lse,  entropy = -sum_j p_j log p_j,  the K largest x_j (ties to the lowest column)
+//     gradient       dx_j = (dlogp ([j = t] - p_j) - dentropy p_j (log p_j + entropy)) / temperature
+//   distill_topk     loss = sum_k q_k (log q_k - (z_{i_k} - lse)), q the teacher's renormalised probabilities; with a
+//                    tail q_k = exp(v_k) and one more term for the bucket of all other columns:
+//                    left (log left - (rest - lse)), left = 1 - sum q, rest = log sum over the other columns exp(z)
+//     gradient       dz_j = W p_j - q_j [j listed] - left exp(z_j - rest) [j not listed],  W = sum q (+ left)
+//
+// The forward kernels read every logit once: a thread keeps a reference value `ref`, S = sum exp2((x - ref) c) and
+// E = sum exp2(t) t with t = (x - ref) c, c = log2(e) / temperature, and moves `ref` up only when a value exceeds it
+// by more than 8 powers of two (floating-point sums lose nothing by a reference that is not the exact maximum). x - ref
+// is formed before the scaling, so that rows of large offsets or of the type's lowest value stay exact. The triples of
+// threads, warps and the CTAs of a cluster are joined by the same rescaling.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "../../include/parpy_b200.h"
+#include "common.cuh"
+#include "cluster.cuh"
+
+namespace {
+
+constexpr double kLn2 = 0.693147180559945309417;
+constexpr double kLog2eD = 1.44269504088896340736;
+constexpr int kTopMax = 128;         // alternatives a row can ask for
+constexpr int kListMax = 1024;       // entries of a teacher's list
+constexpr int kCand = 2048;          // candidates of one selection round
+constexpr int kGroups = 128;         // thread groups whose best values give the selection threshold
+constexpr int kMaxCluster = 8;
+
+using u64 = unsigned long long;
+
+// ---- element types ----------------------------------------------------------------------------
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int VE = 4;
+    static constexpr unsigned kFill = 0xff800000u;   // -inf
+    __device__ static float to_float(float v) { return v; }
+    __device__ static float from_float(float v) { return v; }
+    __device__ static void unpack(const uint4 &r, float (&v)[4]) {
+        v[0] = __uint_as_float(r.x);
+        v[1] = __uint_as_float(r.y);
+        v[2] = __uint_as_float(r.z);
+        v[3] = __uint_as_float(r.w);
+    }
+    __device__ static uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    __device__ static float vmax(const uint4 &r) {
+        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                     fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr int VE = 8;
+    static constexpr unsigned kFill = 0xff80ff80u;
+    __device__ static float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    __device__ static __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+    __device__ static void unpack(const uint4 &r, float (&v)[8]) {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    __device__ static uint4 pack(const float (&v)[8]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned *>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float vmax(const uint4 &r) {
+        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&r);
+        const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
+template <>
+struct Elem<__half> {
+    static constexpr int VE = 8;
+    static constexpr unsigned kFill = 0xfc00fc00u;
+    __device__ static float to_float(__half v) { return __half2float(v); }
+    __device__ static __half from_float(float v) { return __float2half_rn(v); }
+    __device__ static void unpack(const uint4 &r, float (&v)[8]) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(p[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    __device__ static uint4 pack(const float (&v)[8]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned *>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ static float vmax(const uint4 &r) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
+        const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
+
+// ---- packed fp32 pairs (two lanes of one 64-bit register, one instruction each) ------------------------
+__device__ __forceinline__ u64 pack2(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(u64 p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// ---- a row as 16-byte vectors -----------------------------------------------------------------------------
+// Vector v of a row holds the columns [v VE - mis, v VE - mis + VE), where mis is the number of elements between the
+// last 16-byte boundary and the row's start: rows may start at any element. Only the first and the last vector can
+// be partial; they are fetched element by element and filled up with -inf, so nothing outside the row is read.
+template <typename T>
+struct Row {
+    const T *p;
+    int M, mis, nvec, v0, v1;   // vectors [v0, v1) are whole
+    __device__ Row(const T *row, int m) : p(row), M(m) {
+        constexpr int VE = Elem<T>::VE;
+        mis = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+        nvec = (int)(((long long)M + mis + VE - 1) / VE);
+        v0 = mis ? 1 : 0;
+        v1 = (int)(((long long)M + mis) / VE);
+    }
+    __device__ bool whole(int v) const { return v >= v0 && v < v1; }
+    __device__ int first(int v) const { return v * Elem<T>::VE - mis; }
+    __device__ const uint4 *at(int v) const {
+        return reinterpret_cast<const uint4 *>(p + (long long)v * Elem<T>::VE - mis);
+    }
+    __device__ uint4 edge(int v) const {
+        constexpr int VE = Elem<T>::VE;
+        uint4 r = make_uint4(Elem<T>::kFill, Elem<T>::kFill, Elem<T>::kFill, Elem<T>::kFill);
+        T *e = reinterpret_cast<T *>(&r);
+        const int c0 = first(v);
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+            if (c0 + i >= 0 && c0 + i < M) e[i] = p[c0 + i];
+        return r;
+    }
+};
+
+__device__ __forceinline__ uint4 ld_once(const uint4 *p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
+// ---- the order of (value, lowest column) as one 64-bit key: larger is better, 0 is "none" ------------------
+__device__ __forceinline__ unsigned order_of(float f) {
+    const unsigned u = __float_as_uint(f + 0.0f);   // -0 counts as 0
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned o) {
+    return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ u64 key_of(float f, int column) {
+    return ((u64)order_of(f) << 32) | (0xffffffffu - (unsigned)column);
+}
+
+// ---- running softmax sums of one thread ------------------------------------------------------------------------
+struct Sums {
+    float ref, S, E;   // S = 0: nothing finite seen
+};
+
+template <bool ENT>
+__device__ __forceinline__ Sums join(Sums a, float R, float c) {
+    // the sums of `a` relative to the reference R >= a.ref
+    const float r = a.S == 0.0f ? 0.0f : pb::ex2_approx((a.ref - R) * c);
+    Sums o;
+    o.ref = R;
+    o.S = a.S == 0.0f ? 0.0f : a.S * r;
+    o.E = 0.0f;
+    if (ENT) o.E = a.S == 0.0f ? 0.0f : r * (a.E + fmaxf((a.ref - R) * c, -1e30f) * a.S);
+    return o;
+}
+__device__ __forceinline__ float ref_of(const Sums &a) { return a.S == 0.0f ? -INFINITY : a.ref; }
+
+template <bool ENT>
+__device__ __forceinline__ Sums warp_join(Sums a, float c) {
+    const float R = pb::warp_max(ref_of(a));
+    Sums o = join<ENT>(a, R, c);
+    o.S = pb::warp_sum(o.S);
+    if (ENT) o.E = pb::warp_sum(o.E);
+    return o;
+}
+
+enum ListMode { kNone = 0, kRenorm = 1, kTail = 2 };
+
+struct RowArgs {
+    const void *x;
+    long long ldx, N;
+    int M, K;
+    double inv_t;            // 1 / temperature
+    const void *tokens;      // token_logprobs: [N] or null
+    const void *index;       // distill: [N, K]
+    const void *values;      // distill: [N, K]
+    int wide, value_type;    // 64-bit tokens / index; dtype of values
+    float *logp, *lse, *entropy, *top;   // top_logp
+    void *at;                // top_index
+    int at_wide;
+    float *loss, *rest;
+};
+
+__device__ __forceinline__ long long load_index(const void *p, long long i, int wide) {
+    return wide ? static_cast<const long long *>(p)[i] : (long long)static_cast<const int *>(p)[i];
+}
+__device__ __forceinline__ float load_value(const void *p, long long i, int type) {
+    return type == PARPY_B200_F32    ? static_cast<const float *>(p)[i]
+           : type == PARPY_B200_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i])
+                                     : __half2float(static_cast<const __half *>(p)[i]);
+}
+
+// A teacher's list in shared memory. Negative columns and second mentions of a column are not used; a column past the
+// vocabulary makes the row `bad`.
+struct List {
+    int col[kListMax];
+    unsigned char used[kListMax];
+    float v[kListMax], x[kListMax];
+    int bad;
+};
+
+template <typename T>
+__device__ void load_list(List &l, const RowArgs &a, long long row, const T *xr) {
+    if (threadIdx.x == 0) l.bad = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
+        const long long i = load_index(a.index, row * a.K + k, a.wide);
+        const bool in = i >= 0 && i < a.M;
+        if (i >= a.M) l.bad = 1;
+        l.col[k] = in ? (int)i : -1;
+        l.v[k] = load_value(a.values, row * a.K + k, a.value_type);
+        l.x[k] = in ? Elem<T>::to_float(xr[i]) : 0.0f;
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
+        const int c = l.col[k];
+        bool used = c >= 0;
+        for (int j = 0; j < k && used; ++j) used = l.col[j] != c;
+        l.used[k] = used;
+    }
+    __syncthreads();
+}
+
+// What one warp derives from a list: the teacher's normaliser and mass, the student's listed log-mass (natural logs).
+struct Teacher {
+    float norm;       // q_k = exp(v_k - norm)
+    double mass;      // sum q (before `left`), in 64 bits: 1 - mass is next to a border
+    double listed;    // log sum over the listed columns exp(z)
+    int any;          // entries in use
+};
+
+__device__ Teacher warp_teacher(const List &l, int K, bool tail, double inv_t) {
+    const int lane = threadIdx.x & 31;
+    float vm = -INFINITY, xm = -INFINITY;
+    int n = 0;
+    for (int k = lane; k < K; k += 32)
+        if (l.used[k]) {
+            vm = fmaxf(vm, l.v[k]);
+            xm = fmaxf(xm, l.x[k]);
+            ++n;
+        }
+    vm = pb::warp_max(vm);
+    xm = pb::warp_max(xm);
+    const float vref = isinf(vm) ? 0.0f : vm, xref = isinf(xm) ? 0.0f : xm;
+    double sv = 0.0, sx = 0.0;
+    for (int k = lane; k < K; k += 32)
+        if (l.used[k]) {
+            sv += tail ? exp((double)l.v[k]) : (double)expf(l.v[k] - vref);
+            sx += (double)expf((float)(((double)l.x[k] - (double)xref) * inv_t));
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sv += __shfl_xor_sync(0xffffffffu, sv, o);
+        sx += __shfl_xor_sync(0xffffffffu, sx, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    Teacher t;
+    t.any = n;
+    t.norm = tail ? 0.0f : (float)((double)vref + log(sv));
+    if (!tail && sv == 0.0) t.norm = 0.0f;        // no entry with mass: every q is exp(-inf) = 0
+    t.mass = !isfinite(sv) ? (double)NAN : tail ? sv : sv == 0.0 ? 0.0 : 1.0;
+    t.listed = sx == 0.0 ? -INFINITY : (double)xref * inv_t + log(sx);
+    return t;
+}
+
+__device__ __forceinline__ double log_add(double a, double b) {
+    if (a == -INFINITY) return b;
+    if (b == -INFINITY) return a;
+    const double m = fmax(a, b);
+    return m + log(exp(a - m) + exp(b - m));     // NaN stays NaN
+}
+
+// mass of the bucket of all other columns: none where every column is listed
+__device__ __forceinline__ double left_of(const Teacher &t, int M) {
+    const double left = 1.0 - t.mass;
+    return t.any >= M || left < 0.0 ? 0.0 : left;
+}
+
+// Shared memory of the forward kernel. Selection and list parts exist only where they are used.
+template <int THREADS, bool TOP>
+struct TopSmem {};
+template <int THREADS>
+struct TopSmem<THREADS, true> {
+    u64 group[kGroups];
+    u64 cand[kCand];
+    u64 merge[kMaxCluster * kTopMax];
+    int sel[THREADS];
+    u64 tau;
+    int nsel, ncand;
+};
+template <int THREADS, int LIST>
+struct ListSmem {};
+template <int THREADS>
+struct ListSmem<THREADS, kRenorm> {
+    List l;
+};
+template <int THREADS>
+struct ListSmem<THREADS, kTail> {
+    List l;
+    int next[THREADS];
+};
+
+__device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
+// One row per cluster of C CTAs (grid.x = rows x C); vectors dealt round robin to the cluster's threads.
+template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
+__global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(const RowArgs a, const int C) {
+    constexpr int VE = Elem<T>::VE, U = 4, NW = THREADS / 32, GL = THREADS / kGroups;
+    __shared__ Sums s_warp[NW];
+    __shared__ Sums s_rank[kMaxCluster];
+    __shared__ double s_ref, s_log;     // the row's reference value and log(S): lse = ref / temperature + log(S)
+    __shared__ TopSmem<THREADS, TOP> s_top;
+    __shared__ ListSmem<THREADS, LIST> s_list;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+    const long long row = blockIdx.x / C;
+    const int total = C * THREADS, me = rank * THREADS + tid;
+    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
+    const Row<T> rv(xr, a.M);
+    const float c = (float)(kLog2eD * a.inv_t);
+    const float slack = 8.0f / c;
+
+    if constexpr (TOP) {
+        if (C > 1 && rank == 0)
+            for (int i = tid; i < C * a.K; i += THREADS) s_top.merge[i] = 0;
+        if (tid == 0) {
+            s_top.tau = 0;
+            s_top.nsel = 0;
+            s_top.ncand = 0;
+        }
+    }
+    if (C > 1) cluster_arrive();     // matched before the first store into rank 0's shared memory
+    float x_token = 0.0f;
+    long long token = -1;
+    if constexpr (LIST == kNone) {
+        if (rank == 0 && tid == 0 && a.tokens) {
+            token = load_index(a.tokens, row, a.wide);
+            if (token >= 0 && token < a.M) x_token = Elem<T>::to_float(xr[token]);
+        }
+    }
+    int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
+    if constexpr (LIST != kNone) {
+        if constexpr (LIST == kTail) s_list.next[tid] = INT_MAX;
+        load_list(s_list.l, a, row, xr);
+        if constexpr (LIST == kTail) {
+            for (int k = tid; k < a.K; k += THREADS)
+                if (s_list.l.used[k]) {
+                    const int v = (int)(((long long)s_list.l.col[k] + rv.mis) / VE), owner = v % total;
+                    if (owner / THREADS == rank) atomicMin(&s_list.next[owner % THREADS], v);
+                }
+            __syncthreads();
+            next = s_list.next[tid];
+        }
+    }
+
+    float ref = 0.0f, lim = -INFINITY, best = -INFINITY;
+    int best_v = me < rv.nvec ? me : -1;
+    u64 S2 = 0, E2 = 0;
+    const u64 c2 = pack2(c, c);
+
+    auto take = [&](uint4 r, int v) {
+        if constexpr (LIST == kTail) {
+            if (v == next) {         // listed columns are summed apart: read as masked here
+                T *e = reinterpret_cast<T *>(&r);
+                const unsigned fill = Elem<T>::kFill;
+                int after = INT_MAX;
+                for (int k = 0; k < a.K; ++k)
+                    if (s_list.l.used[k]) {
+                        const long long at = (long long)s_list.l.col[k] + rv.mis;
+                        const int w = (int)(at / VE);
+                        if (w == v) {
+                            const int slot = (int)(at - (long long)v * VE);
+#pragma unroll
+                            for (int i = 0; i < VE; ++i)
+                                if (i == slot) e[i] = *reinterpret_cast<const T *>(&fill);
+                        } else if (w > v && w < after && w % total == me) {
+                            after = w;
+                        }
+                    }
+                next = after;
+            }
+        }
+        const float vm = Elem<T>::vmax(r);
+        if constexpr (TOP) {
+            if (vm > best) {
+                best = vm;
+                best_v = v;
+            }
+        }
+        if (vm > lim) {
+            const bool fresh = lim == -INFINITY;         // nothing summed yet: ref means nothing
+            const float sh = fresh ? 0.0f : (ref - vm) * c;
+            const float f = fresh ? 0.0f : pb::ex2_approx(sh);
+            float s0, s1;
+            unpack2(S2, s0, s1);
+            if constexpr (ENT) {
+                float e0, e1;
+                unpack2(E2, e0, e1);
+                const float k = fmaxf(sh, -1e30f);
+                E2 = pack2(f * (e0 + k * s0), f * (e1 + k * s1));
+            }
+            S2 = pack2(f * s0, f * s1);
+            ref = vm;
+            lim = vm + slack;
+        }
+        float f[VE];
+        Elem<T>::unpack(r, f);
+        const u64 nref = pack2(-ref, -ref);
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) {
+            const u64 t = mul2(add2(pack2(f[i], f[i + 1]), nref), c2);
+            float t0, t1;
+            unpack2(t, t0, t1);
+            const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
+            S2 = add2(S2, e);
+            if constexpr (ENT) E2 = fma2(e, pack2(fmaxf(t0, -1e30f), fmaxf(t1, -1e30f)), E2);
+        }
+    };
+
+    if (rv.v0 && me == 0) take(rv.edge(0), 0);
+    {
+        // at most 2^29 + 1 vectors and 2^12 threads: no sum here leaves 32 bits
+        for (int v = me < rv.v0 ? me + total : me; v < rv.v1; v += U * total) {
+            uint4 r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (v + u * total < rv.v1) r[u] = ld_once(rv.at(v + u * total));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (v + u * total < rv.v1) take(r[u], v + u * total);
+        }
+    }
+    if (rv.nvec > rv.v1 && (rv.nvec > 1 || !rv.v0) && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
+
+    Sums mine;
+    {
+        float s0, s1, e0, e1;
+        unpack2(S2, s0, s1);
+        unpack2(E2, e0, e1);
+        mine = {ref, s0 + s1, e0 + e1};
+    }
+    mine = warp_join<ENT>(mine, c);
+    if (lane == 0) s_warp[warp] = mine;
+
+    u64 key = 0;
+    int sub = 0, group = 0;
+    u64 group_key = 0;
+    if constexpr (TOP) {
+        key = best_v < 0 ? 0 : key_of(best, max(rv.first(best_v), 0));
+        group_key = key;
+#pragma unroll
+        for (int o = GL / 2; o > 0; o >>= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, group_key, o);
+            group_key = other > group_key ? other : group_key;
+        }
+        sub = tid % GL;
+        group = tid / GL;
+        if (sub == 0) s_top.group[group] = group_key;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        Sums w = lane < NW ? s_warp[lane] : Sums{0.0f, 0.0f, 0.0f};
+        w = warp_join<ENT>(w, c);
+        if (lane == 0) s_warp[0] = w;
+        __syncwarp();
+    }
+
+    int n_local = 0;
+    if constexpr (TOP) {
+        // A group's best value is one of the row's elements, so the K-th best of the groups' values bounds the K-th
+        // best element from below: only threads whose own best reaches it can hold one of the K. A vector's
+        // place stands for its columns; the bound takes the vector's last column so that it never cuts off a tie.
+        int above = 0;
+        for (int j = sub; j < kGroups; j += GL) above += s_top.group[j] > group_key;
+#pragma unroll
+        for (int o = GL / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (sub == 0 && above == a.K - 1 && group_key != 0) s_top.tau = group_key - (VE - 1);
+        __syncthreads();
+        u64 tau = s_top.tau;
+        if (key != 0 && key >= tau) s_top.sel[atomicAdd(&s_top.nsel, 1)] = tid;
+        __syncthreads();
+        const int per = (rv.nvec + total - 1) / total;
+        const long long items = (long long)s_top.nsel * per;
+        while (true) {
+            for (long long it = tid; it < items; it += THREADS) {
+                const int s = s_top.sel[it / per];
+                const long long v = (long long)rank * THREADS + s + (it % per) * (long long)total;
+                if (v >= rv.nvec) continue;
+                const uint4 r = rv.whole((int)v) ? ld_once(rv.at((int)v)) : rv.edge((int)v);
+                float f[VE];
+                Elem<T>::unpack(r, f);
+                const int c0 = rv.first((int)v);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    const u64 k = key_of(f[i], c0 + i);
+                    if (k >= tau && c0 + i >= 0 && c0 + i < a.M) {
+                        const int p = atomicAdd(&s_top.ncand, 1);
+                        if (p < kCand) s_top.cand[p] = k;
+                    }
+                }
+            }
+            __syncthreads();
+            n_local = s_top.ncand;
+            if (n_local <= kCand) break;
+            // more than fit: the K-th best of any kCand of them is a higher bound, and drops at least kCand - K
+            for (int i = tid; i < kCand; i += THREADS) {
+                const u64 k = s_top.cand[i];
+                int n = 0;
+                for (int j = 0; j < kCand; ++j) n += s_top.cand[j] > k;
+                if (n == a.K - 1) s_top.tau = k;
+            }
+            __syncthreads();
+            tau = s_top.tau;
+            if (tid == 0) s_top.ncand = 0;
+            __syncthreads();
+        }
+    }
+
+    if (C > 1) {
+        cluster_wait();
+        if (tid == 0) {
+            const unsigned to = map_to_rank(smem_u32(&s_rank[rank]), 0);
+            st_cluster_f32(to, s_warp[0].ref);
+            st_cluster_f32(to + 4, s_warp[0].S);
+            st_cluster_f32(to + 8, s_warp[0].E);
+        }
+        if constexpr (TOP) {
+            for (int i = tid; i < n_local; i += THREADS) {
+                const u64 k = s_top.cand[i];
+                int n = 0;
+                for (int j = 0; j < n_local; ++j) n += s_top.cand[j] > k;
+                if (n < a.K) st_cluster_u64(map_to_rank(smem_u32(&s_top.merge[rank * a.K + n]), 0), k);
+            }
+        }
+        cluster_arrive();
+        cluster_wait();
+        if (rank != 0) return;
+    }
+
+    if (warp == 0) {
+        Sums w = C > 1 ? (lane < C ? s_rank[lane] : Sums{0.0f, 0.0f, 0.0f}) : s_warp[0];
+        if (C > 1) w = warp_join<ENT>(w, c);
+        const double S = (double)w.S;
+        double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + log(S);
+        if constexpr (LIST != kNone) {
+            const Teacher t = warp_teacher(s_list.l, a.K, LIST == kTail, a.inv_t);
+            const double rest = lse;
+            if (LIST == kTail) lse = log_add(rest, t.listed);
+            double loss = 0.0;
+            for (int k = lane; k < a.K; k += 32)
+                if (s_list.l.used[k]) {
+                    const double logq = (double)s_list.l.v[k] - (double)t.norm;
+                    const double q = (double)expf((float)logq);
+                    const double z = (double)s_list.l.x[k] * a.inv_t;
+                    if (!(q <= 0.0)) loss += q * (logq - (z == -INFINITY ? z : z - lse));
+                }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+            if (lane == 0) {
+                if (LIST == kTail) {
+                    const double left = left_of(t, a.M);
+                    if (left > 0.0) loss += left * (log(left) - (rest == -INFINITY ? rest : rest - lse));
+                }
+                if (s_list.l.bad || isnan(t.mass)) loss = NAN;
+                a.loss[row] = (float)loss;
+                a.lse[row] = (float)lse;
+                if (a.rest) a.rest[row] = (float)rest;
+            }
+        } else if (lane == 0) {
+            const double logS = log(S);
+            a.lse[row] = (float)lse;
+            // from the difference to ref, so that a large common offset costs nothing
+            if (a.logp)
+                a.logp[row] = token < 0                ? 0.0f
+                              : token >= a.M           ? NAN
+                              : x_token == -INFINITY   ? (isnan(lse) ? NAN : -INFINITY)
+                                                       : (float)(((double)x_token - (double)w.ref) * a.inv_t - logS);
+            if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)(logS - kLn2 * ((double)w.E / S));
+            s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
+            s_log = logS;
+        }
+    }
+    if constexpr (TOP) {
+        __syncthreads();
+        const double row_ref = s_ref, row_log = s_log;
+        const bool broken = isnan(row_ref * 0.0 + row_log);     // S = 0 (log -inf) is an empty row, not a broken one
+        const u64 *from = C > 1 ? s_top.merge : s_top.cand;
+        const int n = C > 1 ? C * a.K : n_local;
+        for (int i = tid; i < n; i += THREADS) {
+            const u64 k = from[i];
+            if (k == 0) continue;
+            int above = 0;
+            for (int j = 0; j < n; ++j) above += from[j] > k;
+            if (above >= a.K) continue;
+            const float v = value_of((unsigned)(k >> 32));
+            const long long o = row * a.K + above;
+            a.top[o] = broken ? NAN : v == -INFINITY ? v : (float)(((double)v - row_ref) * a.inv_t - row_log);
+            const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
+            if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
+            else static_cast<int *>(a.at)[o] = (int)col;
+        }
+    }
+}
+
+// ---- gradients -------------------------------------------------------------------------------------------
+struct GradArgs {
+    RowArgs r;
+    void *dx;
+    long long lddx;
+    const float *lse, *entropy, *rest, *dlogp, *dentropy, *dloss;
+};
+
+// grid.x = rows x parts; the vectors of a row are dealt round robin to the threads of its parts. Every element is
+// read and written by the same thread, so dx may be x itself (a list's logits are read before the first store only
+// within a CTA: in place needs parts = 1 there).
+template <typename T, int THREADS, int LIST>
+__global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int parts) {
+    constexpr int VE = Elem<T>::VE, U = 4;
+    __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kTail> s_list;
+    __shared__ float s_fix[LIST == kNone ? 1 : kListMax];
+    __shared__ Teacher s_teacher;
+    const RowArgs &a = g.r;
+    const int tid = threadIdx.x;
+    const int part = blockIdx.x % parts;
+    const long long row = blockIdx.x / parts;
+    const int total = parts * THREADS, me = part * THREADS + tid;
+    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
+    T *dr = static_cast<T *>(g.dx) + row * g.lddx;
+    const Row<T> rv(xr, a.M);
+    const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15u) == 0;
+    const float c = (float)(kLog2eD * a.inv_t);
+
+    // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the exceptions: the token's
+    // (gamma more) or the listed ones (their value from s_fix). ref is lse (or rest) in units of x, as a high and a
+    // low part, because its rounding would scale the whole row.
+    double base = (double)g.lse[row];
+    float al = 0.0f, be = 0.0f, gamma = 0.0f;
+    int next = INT_MAX, slot = 0;             // the next vector of this thread that holds an exception
+    const bool dead = base == -INFINITY;      // no finite logit in the row: no gradient
+    if constexpr (LIST == kNone) {
+        const long long token = a.tokens ? load_index(a.tokens, row, a.wide) : -1;
+        const double dl = g.dlogp && token >= 0 ? (double)g.dlogp[row] : 0.0;
+        const double de = g.dentropy ? (double)g.dentropy[row] : 0.0;
+        if (!dead) {
+            al = (float)((-dl - (g.dentropy ? de * (double)g.entropy[row] : 0.0)) * a.inv_t);
+            be = (float)(-de * kLn2 * a.inv_t);
+            gamma = (float)(dl * a.inv_t);
+            if (token >= 0 && token < a.M) {
+                next = (int)((token + rv.mis) / VE);
+                slot = (int)((token + rv.mis) % VE);
+            }
+        }
+        if (token >= a.M) al = NAN;
+    } else {
+        s_list.next[tid] = INT_MAX;
+        load_list(s_list.l, a, row, xr);
+        if (tid < 32) {
+            const Teacher t = warp_teacher(s_list.l, a.K, LIST == kTail, a.inv_t);
+            if (tid == 0) s_teacher = t;
+        }
+        for (int k = tid; k < a.K; k += THREADS)
+            if (s_list.l.used[k]) {
+                const int v = (int)(((long long)s_list.l.col[k] + rv.mis) / VE), owner = v % total;
+                if (owner / THREADS == part) atomicMin(&s_list.next[owner % THREADS], v);
+            }
+        __syncthreads();
+        next = s_list.next[tid];
+        const Teacher t = s_teacher;
+        const double w = (double)g.dloss[row] * a.inv_t, lse = base;
+        const double left = LIST == kTail ? left_of(t, a.M) : 0.0, W = t.mass + left;
+        if (!dead) {
+            if (LIST == kTail) {
+                // exp(z - rest) cannot overflow where it is used, however little the student has there
+                base = (double)g.rest[row];
+                al = base == -INFINITY ? 0.0f : (float)(w * (W * exp(base - lse) - left));
+            } else {
+                al = (float)(w * W);
+            }
+        }
+        const bool broken = s_list.l.bad || isnan(t.mass) || isnan(lse);
+        if (broken) al = NAN;
+        for (int k = tid; k < a.K; k += THREADS) {
+            const double z = (double)s_list.l.x[k] * a.inv_t;
+            const float p = z == -INFINITY ? 0.0f : expf((float)(z - lse)), q = expf(s_list.l.v[k] - t.norm);
+            s_fix[k] = broken ? NAN : dead ? 0.0f : (float)(w * (W * (double)p - (double)q));
+        }
+        __syncthreads();
+    }
+    if (base == -INFINITY) base = 0.0;        // every x it meets is -inf: exp2(-inf) = 0
+    base /= a.inv_t;
+    const float hi = (float)base, lo = (float)((base - (double)hi) * (double)c);
+
+    auto put = [&](const uint4 &r, int v, bool whole) {
+        float f[VE];
+        Elem<T>::unpack(r, f);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            const float t = fmaf(f[i] - hi, c, -lo);
+            const float e = pb::ex2_approx(t);
+            f[i] = LIST == kNone ? e * fmaf(be, fmaxf(t, -1e30f), al) : e * al;
+        }
+        if (v == next) {
+            if constexpr (LIST == kNone) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                    if (i == slot) f[i] += gamma;
+            } else {
+                int after = INT_MAX;
+                for (int k = 0; k < a.K; ++k)
+                    if (s_list.l.used[k]) {
+                        const long long at = (long long)s_list.l.col[k] + rv.mis;
+                        const int w = (int)(at / VE);
+                        if (w == v) {
+                            const int s = (int)(at - (long long)v * VE);
+#pragma unroll
+                            for (int i = 0; i < VE; ++i)
+                                if (i == s) f[i] = s_fix[k];
+                        } else if (w > v && w < after && w % total == me) {
+                            after = w;
+                        }
+                    }
+                next = after;
+            }
+        }
+        const int c0 = rv.first(v);
+        if (whole && same) {
+            __stcs(reinterpret_cast<uint4 *>(dr + c0), Elem<T>::pack(f));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+                if (c0 + i >= 0 && c0 + i < a.M) dr[c0 + i] = Elem<T>::from_float(f[i]);
+        }
+    };
+
+    if (rv.v0 && me == 0) put(rv.edge(0), 0, false);
+    for (int v = me < rv.v0 ? me + total : me; v < rv.v1; v += U * total) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v + u * total < rv.v1) r[u] = __ldcs(rv.at(v + u * total));
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v + u * total < rv.v1) put(r[u], v + u * total, true);
+    }
+    if (rv.nvec > rv.v1 && (rv.nvec > 1 || !rv.v0) && me == rv.v1 % total) put(rv.edge(rv.v1), rv.v1, false);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------
+size_t size_of(int32_t dtype) { return dtype == PARPY_B200_F32 ? 4 : 2; }
+
+int32_t check_rows(const char *what, const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                   double temperature) {
+    PB_REQUIRE(dtype == PARPY_B200_F32 || dtype == PARPY_B200_BF16 || dtype == PARPY_B200_F16,
+               "%s: unknown element type %d", what, dtype);
+    PB_REQUIRE(N >= 0 && M >= 1 && M <= INT_MAX - 64, "%s: shape (%lld, %lld) is not supported", what, (long long)N,
+               (long long)M);
+    PB_REQUIRE(ldx >= M || N <= 1, "%s: row pitch %lld is smaller than a row of %lld", what, (long long)ldx,
+               (long long)M);
+    PB_REQUIRE(temperature >= 1e-4 && temperature <= 1e4, "%s: temperature %g is outside [1e-4, 1e4]", what,
+               temperature);
+    PB_REQUIRE(N == 0 || x, "%s: null pointer", what);
+    PB_REQUIRE(reinterpret_cast<uintptr_t>(x) % size_of(dtype) == 0, "%s: misaligned logits", what);
+    return PB_OK;
+}
+
+template <typename K>
+int32_t launch_clustered(K kernel, unsigned grid, unsigned threads, int C, cudaStream_t stream, const RowArgs &a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)C, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    PB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, C));
+    return PB_OK;
+}
+
+template <typename T, bool ENT, bool TOP, int LIST>
+int32_t launch_stats(const char *what, const RowArgs &a, cudaStream_t stream) {
+    pb::DeviceInfo dev;
+    const int32_t rc = pb::device_info(&dev);
+    if (rc) return rc;
+    const long long bytes = (long long)a.M * sizeof(T);
+    const bool big = bytes >= 512 * 16 * 2;
+    const int threads = big ? 512 : 128;
+    int C = 1;
+    while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 16 * 2) C *= 2;
+    PB_REQUIRE(a.N * C <= INT_MAX, "%s: %lld rows are too many", what, a.N);
+    if (big) return launch_clustered(row_stats<T, 512, ENT, TOP, LIST>, (unsigned)(a.N * C), 512, C, stream, a);
+    return launch_clustered(row_stats<T, 128, ENT, TOP, LIST>, (unsigned)(a.N * C), 128, C, stream, a);
+}
+
+template <typename T>
+int32_t launch_logprobs(const RowArgs &a, cudaStream_t stream) {
+    const char *what = "token_logprobs";
+    if (a.entropy)
+        return a.K ? launch_stats<T, true, true, kNone>(what, a, stream)
+                   : launch_stats<T, true, false, kNone>(what, a, stream);
+    return a.K ? launch_stats<T, false, true, kNone>(what, a, stream)
+               : launch_stats<T, false, false, kNone>(what, a, stream);
+}
+
+template <typename T, int LIST>
+int32_t launch_grad(const char *what, const GradArgs &g, cudaStream_t stream) {
+    pb::DeviceInfo dev;
+    const int32_t rc = pb::device_info(&dev);
+    if (rc) return rc;
+    const long long bytes = (long long)g.r.M * sizeof(T);
+    const bool big = bytes >= 512 * 16 * 2, in_place = g.r.x == g.dx;
+    const int threads = big ? 512 : 128;
+    int parts = 1;
+    while (!(LIST != kNone && in_place) && g.r.N * parts < 4LL * dev.sm_count &&
+           bytes / (2 * parts) >= (long long)threads * 16)
+        parts *= 2;
+    PB_REQUIRE(g.r.N * parts <= INT_MAX, "%s: %lld rows are too many", what, g.r.N);
+    const unsigned grid = (unsigned)(g.r.N * parts);
+    if (big) row_grad<T, 512, LIST><<<grid, 512, 0, stream>>>(g, parts);
+    else row_grad<T, 128, LIST><<<grid, 128, 0, stream>>>(g, parts);
+    PB_CUDA(cudaGetLastError());
+    return PB_OK;
+}
+
+int32_t check_gradient(const char *what, const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M, void *dx,
+                       int64_t lddx) {
+    PB_REQUIRE(N == 0 || dx, "%s: null pointer", what);
+    PB_REQUIRE(lddx >= M || N <= 1, "%s: row pitch %lld is smaller than a row of %lld", what, (long long)lddx,
+               (long long)M);
+    PB_REQUIRE(reinterpret_cast<uintptr_t>(dx) % size_of(dtype) == 0, "%s: misaligned gradient", what);
+    PB_REQUIRE(x != dx || ldx == lddx || N <= 1, "%s: in place needs equal row pitches", what);
+    return PB_OK;
+}
+
+int32_t check_list(const char *what, const void *index, const void *values, int32_t value_dtype, int64_t K,
+                   int64_t M) {
+    PB_REQUIRE(index && values, "%s: null pointer", what);
+    PB_REQUIRE(K >= 1 && K <= kListMax, "%s: K=%lld is outside [1, %d]", what, (long long)K, kListMax);
+    PB_REQUIRE(value_dtype == PARPY_B200_F32 || value_dtype == PARPY_B200_BF16 || value_dtype == PARPY_B200_F16,
+               "%s: unknown element type %d", what, value_dtype);
+    (void)M;
+    return PB_OK;
+}
+
+#define PB_BY_TYPE(dtype, expr)                                    \
+    switch (dtype) {                                               \
+        case PARPY_B200_F32: { using T = float; return expr; }     \
+        case PARPY_B200_BF16: { using T = __nv_bfloat16; return expr; } \
+        default: { using T = __half; return expr; }                \
+    }
+
+}  // namespace
+
+extern "C" {
+
+int32_t parpy_b200_token_logprobs(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M, const void *tokens,
+                                  int32_t wide_tokens, double temperature, int64_t K, float *logp, float *lse,
+                                  float *entropy, float *top_logp, void *top_index, int32_t wide_index, void *stream) {
+    const int32_t rc = check_rows("token_logprobs", x, dtype, ldx, N, M, temperature);
+    if (rc) return rc;
+    PB_REQUIRE(K >= 0 && K <= kTopMax && K <= M, "token_logprobs: K=%lld is outside [0, min(M, %d)]", (long long)K,
+               kTopMax);
+    if (N == 0) return PB_OK;
+    PB_REQUIRE(lse && (!logp || tokens) && (K == 0 || (top_logp && top_index)), "token_logprobs: null pointer");
+    RowArgs a = {};
+    a.x = x;
+    a.ldx = ldx;
+    a.N = N;
+    a.M = (int)M;
+    a.K = (int)K;
+    a.inv_t = 1.0 / temperature;
+    a.tokens = logp ? tokens : nullptr;
+    a.wide = wide_tokens;
+    a.logp = logp;
+    a.lse = lse;
+    a.entropy = entropy;
+    a.top = top_logp;
+    a.at = top_index;
+    a.at_wide = wide_index;
+    PB_BY_TYPE(dtype, launch_logprobs<T>(a, static_cast<cudaStream_t>(stream)))
+}
+
+int32_t parpy_b200_token_logprobs_grad(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                       const void *tokens, int32_t wide_tokens, double temperature, const float *lse,
+                                       const float *entropy, const float *dlogp, const float *dentropy, void *dx,
+                                       int64_t lddx, void *stream) {
+    int32_t rc = check_rows("token_logprobs_grad", x, dtype, ldx, N, M, temperature);
+    if (!rc) rc = check_gradient("token_logprobs_grad", x, dtype, ldx, N, M, dx, lddx);
+    if (rc || N == 0) return rc;
+    PB_REQUIRE(lse && (!dlogp || tokens) && (!dentropy || entropy), "token_logprobs_grad: null pointer");
+    GradArgs g = {};
+    g.r.x = x;
+    g.r.ldx = ldx;
+    g.r.N = N;
+    g.r.M = (int)M;
+    g.r.inv_t = 1.0 / temperature;
+    g.r.tokens = dlogp ? tokens : nullptr;
+    g.r.wide = wide_tokens;
+    g.dx = dx;
+    g.lddx = lddx;
+    g.lse = lse;
+    g.entropy = entropy;
+    g.dlogp = dlogp;
+    g.dentropy = dentropy;
+    PB_BY_TYPE(dtype, (launch_grad<T, kNone>("token_logprobs_grad", g, static_cast<cudaStream_t>(stream))))
+}
+
+int32_t parpy_b200_distill_topk(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M, const void *index,
+                                int32_t wide_index, const void *values, int32_t value_dtype, int64_t K,
+                                double temperature, int32_t tail, float *loss, float *lse, float *rest, void *stream) {
+    int32_t rc = check_rows("distill_topk", x, dtype, ldx, N, M, temperature);
+    if (rc || N == 0) return rc;
+    rc = check_list("distill_topk", index, values, value_dtype, K, M);
+    if (rc) return rc;
+    PB_REQUIRE(loss && lse && (!tail || rest), "distill_topk: null pointer");
+    RowArgs a = {};
+    a.x = x;
+    a.ldx = ldx;
+    a.N = N;
+    a.M = (int)M;
+    a.K = (int)K;
+    a.inv_t = 1.0 / temperature;
+    a.index = index;
+    a.values = values;
+    a.wide = wide_index;
+    a.value_type = value_dtype;
+    a.lse = lse;
+    a.loss = loss;
+    a.rest = tail ? rest : nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    PB_BY_TYPE(dtype, (tail ? launch_stats<T, false, false, kTail>("distill_topk", a, s)
+                            : launch_stats<T, false, false, kRenorm>("distill_topk", a, s)))
+}
+
+int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
+                                     const void *index, int32_t wide_index, const void *values, int32_t value_dtype,
+                                     int64_t K, double temperature, int32_t tail, const float *lse, const float *rest,
+                                     const float *dloss, void *dx, int64_t lddx, void *stream) {
+    int32_t rc = check_rows("distill_topk_grad", x, dtype, ldx, N, M, temperature);
+    if (!rc) rc = check_gradient("distill_topk_grad", x, dtype, ldx, N, M, dx, lddx);
+    if (rc || N == 0) return rc;
+    rc = check_list("distill_topk_grad", index, values, value_dtype, K, M);
+    if (rc) return rc;
+    PB_REQUIRE(lse && dloss && (!tail || rest), "distill_topk_grad: null pointer");
+    GradArgs g = {};
+    g.r.x = x;
+    g.r.ldx = ldx;
+    g.r.N = N;
+    g.r.M = (int)M;
+    g.r.K = (int)K;
+    g.r.inv_t = 1.0 / temperature;
+    g.r.index = index;
+    g.r.values = values;
+    g.r.wide = wide_index;
+    g.r.value_type = value_dtype;
+    g.dx = dx;
+    g.lddx = lddx;
+    g.lse = lse;
+    g.rest = rest;
+    g.dloss = dloss;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    PB_BY_TYPE(dtype, (tail ? launch_grad<T, kTail>("distill_topk_grad", g, s)
+                            : launch_grad<T, kRenorm>("distill_topk_grad", g, s)))
+}
+
+}  // extern "C"

@@ -4,7 +4,12 @@ to their native kernels under the reference's names and signatures: ``softmax``
 (test/test_reduce.py:12-70), ``spmv_row`` (test/test_spmv.py:12-18) and the
 SDDMM kernels (benchmarks/sddmm.py:21-41,63-70). All take ``opts=`` and write
 their outputs in place. ``sum_max`` is this package's fused one-pass sum + max
-of a long vector."""
+of a long vector.
+
+Beside them stand operators of language models on the same kinds of data: on rows of
+vocabulary logits ``token_logprobs`` and ``distill_topk`` with their gradients. They take
+float32, bfloat16 and float16 and, for CUDA arrays, rows that lie apart (a slice of a wider
+matrix); arguments that may be ``None`` are named in their docstrings."""
 from . import jit
 
 
@@ -75,3 +80,37 @@ def sum_exp_3d(x, N, M, out):
 @jit
 def spmm_cell(A, B, C):
     """C[i,j] += sum over row i's non-zeros of A.values[a] * B.values[A.cols[a], j]"""
+
+
+@jit
+def token_logprobs(x, tokens, N, M, K, temperature, logp, lse, entropy, top_logp, top_index):
+    """For every row of logits x[N,M], with z = x / temperature: lse = log(sum(exp(z))),
+    logp = z[tokens] - lse (0 for a negative token, NaN for one past the row), the
+    entropy of softmax(z), and the K (at most 128) largest columns in falling order, ties by the lowest:
+    their log-probabilities top_logp[N,K] and numbers top_index[N,K]. A logit of -inf is a column that a
+    mask took out; a row of nothing else has lse and logp -inf and entropy 0; a row with a
+    NaN or +inf gets NaN (top_index -1). ``tokens`` with ``logp``, ``entropy``, and for K = 0 ``top_logp``
+    and ``top_index`` may be None. lse (and entropy) are what the gradient needs."""
+
+
+@jit
+def token_logprobs_grad(x, tokens, N, M, temperature, lse, entropy, dlogp, dentropy, dx):
+    """dx[N,M] = gradient of sum(dlogp * logp + dentropy * entropy) with respect to x, in x's
+    type; dx may be x. ``dlogp`` (then ``tokens``) and ``dentropy`` (then ``entropy``) may be None.
+    The alternatives are reported, not differentiated. A row without a finite logit gets zeros."""
+
+
+@jit
+def distill_topk(x, index, values, N, M, K, temperature, tail, loss, lse, rest):
+    """loss[N] = distance of the student's softmax(x / temperature) from a teacher known by its K (at most 1024)
+    best columns index[N,K] and their logits or log-probabilities values[N,K], at the temperature wanted
+    (what ``token_logprobs`` gives as top_index and top_logp). Without ``tail`` the teacher's
+    probabilities are renormalised over the list: sum(q * (log(q) - log(p))). With it q = exp(values),
+    and the mass that the list leaves is compared with the student's mass outside the list. A
+    negative index is an entry not given, a column's second mention is not used, an index past the row
+    makes it NaN. Also writes lse[N] and, with a tail, rest[N] (else None), which the gradient needs."""
+
+
+@jit
+def distill_topk_grad(x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
+    """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x."""

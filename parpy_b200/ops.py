@@ -12,6 +12,9 @@ memory:
   inout   copied both ways
   skip    not staged at all (scratch the native kernel ignores)
 
+A role that ends in ``_rows`` says that the kernel takes the strides of a CUDA array: its
+last dimension is contiguous, the others may be a slice of something larger.
+
 and an adapter that flattens the arguments the way the reference's ctypes
 wrapper does (python/parpy/compile.py:140-178) and calls the C ABI on torch's
 current stream.
@@ -82,6 +85,14 @@ def scalar(v, what):
     raise TypeError(f"{what}: expected an int, float or 0-d array, got {type(v)}")
 
 
+def given(v, what, shape, dtype, allow_none=False):
+    """The CUDA tensor behind an argument of exactly this shape, or None for None where that is allowed."""
+    t = tensor(v, what, dtype, len(shape), allow_none)
+    if t is not None and tuple(t.shape) != shape:
+        raise RuntimeError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
+    return t
+
+
 def tensor(v, what, dtype=None, ndim=None, allow_none=False):
     """The CUDA torch tensor behind a buffer argument, with dtype/rank checks."""
     if v is None:
@@ -112,6 +123,24 @@ def ptr(t):
 def current_stream():
     import torch
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _float_types():
+    import torch
+    return {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+
+
+def _pitch(t, what, output=False):
+    """Strides of every dimension but the last of an array that is contiguous along its last."""
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous, got strides {t.stride()}")
+    if output:
+        reach = t.shape[-1]
+        for n, s in sorted(zip(t.shape[:-1], t.stride()[:-1]), key=lambda d: d[1]):
+            if n > 1 and s < reach:
+                raise ValueError(f"{what}: rows of an output must not overlap, got strides {t.stride()}")
+            reach = max(reach, s * (n - 1) + reach)
+    return tuple(t.stride()[:-1])
 
 
 # ---- HMM forward ---------------------------------------------------------------
@@ -382,3 +411,117 @@ register(OpSpec("spmm_cell", ("A", "B", "C"),
                 {"A": {"values": "in", "rows": "in", "cols": "in", "nrows": "in"},
                  "B": {"values": "in", "ncols": "in"}, "C": "inout"},
                 _spmm_call, doc="test/test_spmm.py:16-24"))
+
+
+# ---- rows of vocabulary logits -------------------------------------------------------------------
+def _logits(fun, x, N, M, what="x", like=None, output=False):
+    """(tensor, dtype code, row pitch, N, M) of a matrix of logits."""
+    n, m = int(scalar(N, "N")), int(scalar(M, "M"))
+    types = _float_types()
+    t = given(x, f"{fun}: {what}", (n, m), like.dtype if like is not None else tuple(types))
+    if m < 1:
+        raise RuntimeError(f"{fun}: needs at least one column, got M={m}")
+    (pitch,) = _pitch(t, f"{fun}: {what}", output)
+    return t, types[t.dtype], max(pitch, m) if n <= 1 else pitch, n, m
+
+
+def _temperature(fun, temperature):
+    t = float(scalar(temperature, "temperature"))
+    if not 1e-4 <= t <= 1e4:
+        raise RuntimeError(f"{fun}: temperature {t:g} is outside [1e-4, 1e4]")
+    return t
+
+
+def _wide(t):
+    import torch
+    return int(t is not None and t.dtype == torch.int64)
+
+
+def _token_logprobs_call(opts, x, tokens, N, M, K, temperature, logp, lse, entropy, top_logp, top_index):
+    import torch
+    f, f32, whole = "token_logprobs", torch.float32, (torch.int64, torch.int32)
+    xt, dtype, ld, n, m = _logits(f, x, N, M)
+    k = int(scalar(K, "K"))
+    if not 0 <= k <= min(m, _native.TOP_MAX):
+        raise RuntimeError(f"{f}: K={k} is outside [0, {min(m, _native.TOP_MAX)}]")
+    tok = given(tokens, f"{f}: tokens", (n,), whole, allow_none=logp is None)
+    lp = given(logp, f"{f}: logp", (n,), f32, allow_none=True)
+    ls = given(lse, f"{f}: lse", (n,), f32)
+    en = given(entropy, f"{f}: entropy", (n,), f32, allow_none=True)
+    tl = given(top_logp, f"{f}: top_logp", (n, k), f32) if k else None
+    ti = given(top_index, f"{f}: top_index", (n, k), whole) if k else None
+    _native.check(_native.lib().parpy_b200_token_logprobs(
+        ptr(xt), dtype, ld, n, m, ptr(tok), _wide(tok), _temperature(f, temperature), k, ptr(lp), ptr(ls), ptr(en),
+        ptr(tl), ptr(ti), _wide(ti), current_stream()), f)
+
+
+def _token_logprobs_grad_call(opts, x, tokens, N, M, temperature, lse, entropy, dlogp, dentropy, dx):
+    import torch
+    f, f32, whole = "token_logprobs_grad", torch.float32, (torch.int64, torch.int32)
+    xt, dtype, ld, n, m = _logits(f, x, N, M)
+    dt, _, ldd, _, _ = _logits(f, dx, N, M, "dx", like=xt, output=True)
+    tok = given(tokens, f"{f}: tokens", (n,), whole, allow_none=dlogp is None)
+    ls = given(lse, f"{f}: lse", (n,), f32)
+    dl = given(dlogp, f"{f}: dlogp", (n,), f32, allow_none=True)
+    de = given(dentropy, f"{f}: dentropy", (n,), f32, allow_none=True)
+    en = given(entropy, f"{f}: entropy", (n,), f32, allow_none=de is None)
+    _native.check(_native.lib().parpy_b200_token_logprobs_grad(
+        ptr(xt), dtype, ld, n, m, ptr(tok), _wide(tok), _temperature(f, temperature), ptr(ls), ptr(en), ptr(dl),
+        ptr(de), ptr(dt), ldd, current_stream()), f)
+
+
+register(OpSpec("token_logprobs",
+                ("x", "tokens", "N", "M", "K", "temperature", "logp", "lse", "entropy", "top_logp", "top_index"),
+                {"x": "in_rows", "tokens": "in", "logp": "out", "lse": "out", "entropy": "out", "top_logp": "out",
+                 "top_index": "out"}, _token_logprobs_call, doc="log-probabilities, entropy and alternatives"))
+register(OpSpec("token_logprobs_grad",
+                ("x", "tokens", "N", "M", "temperature", "lse", "entropy", "dlogp", "dentropy", "dx"),
+                {"x": "in_rows", "dx": "out_rows"}, _token_logprobs_grad_call, doc="gradient of token_logprobs"))
+
+
+def _teacher(f, index, values, n, K):
+    import torch
+    k = int(scalar(K, "K"))
+    if not 1 <= k <= _native.LIST_MAX:
+        raise RuntimeError(f"{f}: K={k} is outside [1, {_native.LIST_MAX}]")
+    it = given(index, f"{f}: index", (n, k), (torch.int64, torch.int32))
+    vt = given(values, f"{f}: values", (n, k), tuple(_float_types()))
+    return it, vt, _float_types()[vt.dtype], k
+
+
+def _distill_topk_call(opts, x, index, values, N, M, K, temperature, tail, loss, lse, rest):
+    import torch
+    f, f32 = "distill_topk", torch.float32
+    xt, dtype, ld, n, m = _logits(f, x, N, M)
+    it, vt, vtype, k = _teacher(f, index, values, n, K)
+    bucket = int(bool(scalar(tail, "tail")))
+    lo = given(loss, f"{f}: loss", (n,), f32)
+    ls = given(lse, f"{f}: lse", (n,), f32)
+    re = given(rest, f"{f}: rest", (n,), f32, allow_none=not bucket)
+    _native.check(_native.lib().parpy_b200_distill_topk(
+        ptr(xt), dtype, ld, n, m, ptr(it), _wide(it), ptr(vt), vtype, k, _temperature(f, temperature), bucket, ptr(lo),
+        ptr(ls), ptr(re), current_stream()), f)
+
+
+def _distill_topk_grad_call(opts, x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
+    import torch
+    f, f32 = "distill_topk_grad", torch.float32
+    xt, dtype, ld, n, m = _logits(f, x, N, M)
+    dt, _, ldd, _, _ = _logits(f, dx, N, M, "dx", like=xt, output=True)
+    it, vt, vtype, k = _teacher(f, index, values, n, K)
+    bucket = int(bool(scalar(tail, "tail")))
+    ls = given(lse, f"{f}: lse", (n,), f32)
+    re = given(rest, f"{f}: rest", (n,), f32, allow_none=not bucket)
+    dl = given(dloss, f"{f}: dloss", (n,), f32)
+    _native.check(_native.lib().parpy_b200_distill_topk_grad(
+        ptr(xt), dtype, ld, n, m, ptr(it), _wide(it), ptr(vt), vtype, k, _temperature(f, temperature), bucket, ptr(ls),
+        ptr(re), ptr(dl), ptr(dt), ldd, current_stream()), f)
+
+
+register(OpSpec("distill_topk",
+                ("x", "index", "values", "N", "M", "K", "temperature", "tail", "loss", "lse", "rest"),
+                {"x": "in_rows", "loss": "out", "lse": "out", "rest": "out"}, _distill_topk_call,
+                doc="distance to a teacher known by its best columns"))
+register(OpSpec("distill_topk_grad",
+                ("x", "index", "values", "N", "M", "K", "temperature", "tail", "lse", "rest", "dloss", "dx"),
+                {"x": "in_rows", "dx": "out_rows"}, _distill_topk_grad_call, doc="gradient of distill_topk"))

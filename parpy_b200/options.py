@@ -36,6 +36,7 @@ class ElemSize(enum.Enum):
     U32 = "u4"
     U64 = "u8"
     F16 = "f2"
+    BF16 = "V2"     # torch's typestr for bfloat16, which NumPy has no type for
     F32 = "f4"
     F64 = "f8"
 
@@ -55,9 +56,11 @@ class ElemSize(enum.Enum):
         return self.value[0] == "u"
 
     def is_floating_point(self):
-        return self.value[0] == "f"
+        return self.value[0] in "fV"
 
     def to_numpy(self):
+        if self is ElemSize.BF16:
+            raise RuntimeError("NumPy has no bfloat16 type")
         return {"b1": np.bool_, "i1": np.int8, "i2": np.int16, "i4": np.int32, "i8": np.int64,
                 "u1": np.uint8, "u2": np.uint16, "u4": np.uint32, "u8": np.uint64,
                 "f2": np.float16, "f4": np.float32, "f8": np.float64}[self.value]
@@ -68,14 +71,14 @@ class ElemSize(enum.Enum):
         import torch
         return {"b1": torch.bool, "i1": torch.int8, "i2": torch.int16, "i4": torch.int32,
                 "i8": torch.int64, "u1": torch.uint8, "u2": torch.int16, "u4": torch.int32,
-                "u8": torch.int64, "f2": torch.float16, "f4": torch.float32,
+                "u8": torch.int64, "f2": torch.float16, "V2": torch.bfloat16, "f4": torch.float32,
                 "f8": torch.float64}[self.value]
 
     def to_ctype(self):
         return {"b1": ctypes.c_bool, "i1": ctypes.c_int8, "i2": ctypes.c_int16,
                 "i4": ctypes.c_int32, "i8": ctypes.c_int64, "u1": ctypes.c_uint8,
                 "u2": ctypes.c_uint16, "u4": ctypes.c_uint32, "u8": ctypes.c_uint64,
-                "f2": ctypes.c_uint16, "f4": ctypes.c_float, "f8": ctypes.c_double}[self.value]
+                "f2": ctypes.c_uint16, "V2": ctypes.c_uint16, "f4": ctypes.c_float, "f8": ctypes.c_double}[self.value]
 
 
 class DataType:

@@ -36,6 +36,8 @@ KERNEL_FILES = {
     "spmv_row": "sparse.cu", "spmm_cell": "sparse.cu",
     "parpy_sddmm_decompress_csr": "sparse.cu", "parpy_sddmm_csr_kernel": "sparse.cu",
     "parpy_sddmm_coo_kernel": "sparse.cu",
+    "token_logprobs": "logits.cu", "token_logprobs_grad": "logits.cu",
+    "distill_topk": "logits.cu", "distill_topk_grad": "logits.cu",
 }
 for _op in ("sum", "prod", "max", "min"):
     for _kind in ("rows", "axis", "2d"):
@@ -60,7 +62,7 @@ def kernel_source(op_name):
     parts = [f"// parpy_b200: amalgamated source for '{op_name}' (sm_100a)\n"
              f"// build: nvcc -std=c++17 -O3 -gencode arch=compute_100a,code=sm_100a -shared -Xcompiler -fPIC\n"]
     files = [_HEADER, _CSRC / "common.cuh"]
-    if KERNEL_FILES[op_name].startswith("hmm_"):
+    if KERNEL_FILES[op_name].startswith(("hmm_", "logits")):
         files.append(_CSRC / "cluster.cuh")
     files += [_CSRC / "runtime.cu", _CSRC / KERNEL_FILES[op_name]]
     for path in files:

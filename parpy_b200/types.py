@@ -11,6 +11,7 @@ U16 = ElemSize.U16
 U32 = ElemSize.U32
 U64 = ElemSize.U64
 F16 = ElemSize.F16
+BF16 = ElemSize.BF16
 F32 = ElemSize.F32
 F64 = ElemSize.F64
 
