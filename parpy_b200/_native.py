@@ -80,11 +80,18 @@ SIGNATURES = {
                                         c_i32, c_ptr, c_ptr, c_ptr, c_ptr]),
     "parpy_b200_distill_topk_grad": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_i64,
                                              c_f64, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
+    "parpy_b200_gated_scan": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32,
+                                      c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "parpy_b200_gated_scan_grad": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr,
+                                           c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "parpy_b200_gated_step": (c_i32, [c_i32, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr,
+                                      c_ptr]),
 }
 
 # element types, and the most alternatives / list entries of a row, of the logits entries
 F32, BF16, F16 = 0, 1, 2
 TOP_MAX, LIST_MAX = 128, 1024
+SCAN_TILE = 128      # steps between the states that gated_scan stores for its gradient
 
 REDUCE_SUM, REDUCE_PROD, REDUCE_MAX, REDUCE_MIN = 0, 1, 2, 3
 

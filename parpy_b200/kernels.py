@@ -7,10 +7,11 @@ their outputs in place. ``sum_max`` is this package's fused one-pass sum + max
 of a long vector.
 
 Beside them stand operators of language models on the same kinds of data: on rows of
-vocabulary logits ``token_logprobs`` and ``distill_topk`` with their gradients. They take
-float32, bfloat16 and float16 and, for CUDA arrays, rows that lie apart (a slice of a wider
+vocabulary logits ``token_logprobs`` and ``distill_topk`` with their gradients; over
+padded sequences the recurrence ``gated_scan`` with its gradient and, for decoding, ``gated_step``. They take float32, bfloat16 and float16 and, for CUDA arrays, rows that lie apart (a slice of a wider
 matrix); arguments that may be ``None`` are named in their docstrings."""
 from . import jit
+from ._native import SCAN_TILE
 
 
 @jit
@@ -114,3 +115,24 @@ def distill_topk(x, index, values, N, M, K, temperature, tail, loss, lse, rest):
 @jit
 def distill_topk_grad(x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
     """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x."""
+
+
+@jit
+def gated_scan(g, x, h0, lens, B, T, D, h, last, carry):
+    """For every sequence and channel of g, x [B,T,D]: f = sigmoid(g), h[t] = f[t] * h[t-1] + (1 - f[t]) * x[t]
+    from the state h0[B,D] (None: zeros), in 32 bits, h rounded once to the type of x. From lens[b]
+    (None: T; clamped to [0, T]) on the state is held and h is zero. ``last`` [B,D] (or None) is the final state,
+    ``carry`` [B,ceil(T/SCAN_TILE),D] (or None) the states that ``gated_scan_grad`` starts from; both float32,
+    as h0. CUDA arrays g, x, h may be strided between sequences and between steps."""
+
+
+@jit
+def gated_scan_grad(g, x, lens, B, T, D, carry, dh, dlast, dg, dx, dh0):
+    """dg, dx [B,T,D] and dh0 [B,D] (or None) = gradients of sum(dh * h) + sum(dlast * last); dh or dlast
+    may be None. ``carry`` is what ``gated_scan`` wrote for the same inputs. dg and dx are zero from lens[b] on."""
+
+
+@jit
+def gated_step(g, x, state, N, D, h, last):
+    """One step for N rows: last = sigmoid(g) * state + (1 - sigmoid(g)) * x in float32 (last may be
+    state), h[N,D] the same in the type of x."""

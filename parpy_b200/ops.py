@@ -525,3 +525,80 @@ register(OpSpec("distill_topk",
 register(OpSpec("distill_topk_grad",
                 ("x", "index", "values", "N", "M", "K", "temperature", "tail", "lse", "rest", "dloss", "dx"),
                 {"x": "in_rows", "dx": "out_rows"}, _distill_topk_grad_call, doc="gradient of distill_topk"))
+
+
+# ---- gated linear recurrence ------------------------------------------------------------------------
+def _steps(f, name, a, shape, like=None, output=False, allow_none=False):
+    """(tensor, its two strides as a host array) of one [B, T, D] argument."""
+    t = given(a, f"{f}: {name}", shape, like.dtype if like is not None else tuple(_float_types()), allow_none)
+    if t is None:
+        return None, None
+    return t, (ctypes.c_int64 * 2)(*_pitch(t, f"{f}: {name}", output))
+
+
+def _scan_shape(f, B, T, D):
+    b, t, d = (int(scalar(v, n)) for v, n in ((B, "B"), (T, "T"), (D, "D")))
+    if min(b, t, d) < 0:
+        raise RuntimeError(f"{f}: negative shape {(b, t, d)}")
+    return b, t, d
+
+
+def _gated_scan_call(opts, g, x, h0, lens, B, T, D, h, last, carry):
+    import torch
+    f, f32 = "gated_scan", torch.float32
+    b, t, d = _scan_shape(f, B, T, D)
+    gt, gs = _steps(f, "g", g, (b, t, d))
+    xt, xs = _steps(f, "x", x, (b, t, d), gt)
+    ht, hs = _steps(f, "h", h, (b, t, d), gt, output=True)
+    first = given(h0, f"{f}: h0", (b, d), f32, allow_none=True)
+    n = given(lens, f"{f}: lens", (b,), (torch.int64, torch.int32), allow_none=True)
+    end = given(last, f"{f}: last", (b, d), f32, allow_none=True)
+    kept = given(carry, f"{f}: carry", (b, -(-t // _native.SCAN_TILE), d), f32, allow_none=True)
+    _native.check(_native.lib().parpy_b200_gated_scan(
+        _float_types()[gt.dtype], b, t, d, ptr(gt), gs, ptr(xt), xs, ptr(first), ptr(n), _wide(n), ptr(ht), hs,
+        ptr(end), ptr(kept), current_stream()), f)
+
+
+def _gated_scan_grad_call(opts, g, x, lens, B, T, D, carry, dh, dlast, dg, dx, dh0):
+    import torch
+    f, f32 = "gated_scan_grad", torch.float32
+    b, t, d = _scan_shape(f, B, T, D)
+    gt, gs = _steps(f, "g", g, (b, t, d))
+    xt, xs = _steps(f, "x", x, (b, t, d), gt)
+    dt, ds = _steps(f, "dh", dh, (b, t, d), gt, allow_none=True)
+    dgt, dgs = _steps(f, "dg", dg, (b, t, d), gt, output=True)
+    dxt, dxs = _steps(f, "dx", dx, (b, t, d), gt, output=True)
+    n = given(lens, f"{f}: lens", (b,), (torch.int64, torch.int32), allow_none=True)
+    kept = given(carry, f"{f}: carry", (b, -(-t // _native.SCAN_TILE), d), f32)
+    end = given(dlast, f"{f}: dlast", (b, d), f32, allow_none=True)
+    first = given(dh0, f"{f}: dh0", (b, d), f32, allow_none=True)
+    _native.check(_native.lib().parpy_b200_gated_scan_grad(
+        _float_types()[gt.dtype], b, t, d, ptr(gt), gs, ptr(xt), xs, ptr(n), _wide(n), ptr(kept), ptr(dt), ds,
+        ptr(end), ptr(dgt), dgs, ptr(dxt), dxs, ptr(first), current_stream()), f)
+
+
+def _gated_step_call(opts, g, x, state, N, D, h, last):
+    import torch
+    f, f32 = "gated_step", torch.float32
+    n, d = int(scalar(N, "N")), int(scalar(D, "D"))
+    gt = given(g, f"{f}: g", (n, d), tuple(_float_types()))
+    xt = given(x, f"{f}: x", (n, d), gt.dtype)
+    ht = given(h, f"{f}: h", (n, d), gt.dtype)
+    before = given(state, f"{f}: state", (n, d), f32)
+    after = given(last, f"{f}: last", (n, d), f32)
+    (lg,), (lx,), (lh,) = (_pitch(a, f"{f}: {w}", w == "h") for a, w in ((gt, "g"), (xt, "x"), (ht, "h")))
+    _native.check(_native.lib().parpy_b200_gated_step(
+        _float_types()[gt.dtype], n, d, ptr(gt), lg, ptr(xt), lx, ptr(before), ptr(ht), lh, ptr(after),
+        current_stream()), f)
+
+
+register(OpSpec("gated_scan", ("g", "x", "h0", "lens", "B", "T", "D", "h", "last", "carry"),
+                {"g": "in_rows", "x": "in_rows", "h": "out_rows", "last": "out", "carry": "inout"}, _gated_scan_call,
+                doc="gated linear recurrence over padded sequences"))
+register(OpSpec("gated_scan_grad",
+                ("g", "x", "lens", "B", "T", "D", "carry", "dh", "dlast", "dg", "dx", "dh0"),
+                {"g": "in_rows", "x": "in_rows", "dh": "in_rows", "dg": "out_rows", "dx": "out_rows", "dh0": "out"},
+                _gated_scan_grad_call, doc="gradient of gated_scan"))
+register(OpSpec("gated_step", ("g", "x", "state", "N", "D", "h", "last"),
+                {"g": "in_rows", "x": "in_rows", "h": "out_rows", "last": "out"}, _gated_step_call,
+                doc="one step of gated_scan for a decoding batch"))

@@ -38,6 +38,7 @@ KERNEL_FILES = {
     "parpy_sddmm_coo_kernel": "sparse.cu",
     "token_logprobs": "logits.cu", "token_logprobs_grad": "logits.cu",
     "distill_topk": "logits.cu", "distill_topk_grad": "logits.cu",
+    "gated_scan": "recurrence.cu", "gated_scan_grad": "recurrence.cu", "gated_step": "recurrence.cu",
 }
 for _op in ("sum", "prod", "max", "min"):
     for _kind in ("rows", "axis", "2d"):
@@ -62,7 +63,7 @@ def kernel_source(op_name):
     parts = [f"// parpy_b200: amalgamated source for '{op_name}' (sm_100a)\n"
              f"// build: nvcc -std=c++17 -O3 -gencode arch=compute_100a,code=sm_100a -shared -Xcompiler -fPIC\n"]
     files = [_HEADER, _CSRC / "common.cuh"]
-    if KERNEL_FILES[op_name].startswith(("hmm_", "logits")):
+    if KERNEL_FILES[op_name].startswith(("hmm_", "logits", "recurrence")):
         files.append(_CSRC / "cluster.cuh")
     files += [_CSRC / "runtime.cu", _CSRC / KERNEL_FILES[op_name]]
     for path in files:
