@@ -388,26 +388,24 @@ int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, 
 /* ---- gated linear recurrence ----------------------------------------------------------------
  * No counterpart in the reference; its nearest function is the recurrence over observation
  * sequences of benchmarks/forward.py:94-187. f = sigmoid(g), h_t = f_t h_{t-1} + (1 - f_t) x_t for
- * every channel of g, x [B, T, D] (element type `dtype`: PARPY_B200_F32, _BF16, _F16). Strides are host
- * arrays of two numbers, the elements between sequences and between steps; channels are
- * contiguous. States are kept in 32 bits: h0[B, D] (NULL: zeros), last[B, D] (NULL: not written), and
+ * every channel of g, x [B, T, D] (element type `dtype`: PARPY_B200_F32, _BF16, _F16). _sb and _st are the
+ * elements between sequences and between steps of an array; channels are contiguous. States are kept in 32 bits: h0[B, D] (NULL: zeros), last[B, D] (NULL: not written), and
  * carry[B, ceil(T / PARPY_B200_SCAN_TILE), D], the state that enters each run of
  * PARPY_B200_SCAN_TILE steps, which the gradient starts from (NULL where none is wanted).
  * lens[B] (NULL: all T; 64-bit where wide_lens is set; values outside [0, T] count as the nearest):
  * from lens[b] on the state is held, h, dg and dx are zero, and g, x, dh are not read. */
 #define PARPY_B200_SCAN_TILE 128
-int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g,
-                              const int64_t *g_strides, const void *x, const int64_t *x_strides, const float *h0,
-                              const void *lens, int32_t wide_lens, void *h, const int64_t *h_strides, float *last,
+int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
+                              int64_t g_st, const void *x, int64_t x_sb, int64_t x_st, const float *h0,
+                              const void *lens, int32_t wide_lens, void *h, int64_t h_sb, int64_t h_st, float *last,
                               float *carry, void *stream);
 /* Gradients dg, dx [B, T, D] and dh0[B, D] (NULL: not written) of sum(dh h) + sum(dlast last); dh or
  * dlast may be NULL: no such term. carry is what gated_scan wrote for the same g, x, h0, lens. */
-int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g,
-                                   const int64_t *g_strides, const void *x, const int64_t *x_strides,
-                                   const void *lens, int32_t wide_lens, const float *carry, const void *dh,
-                                   const int64_t *dh_strides, const float *dlast, void *dg,
-                                   const int64_t *dg_strides, void *dx, const int64_t *dx_strides, float *dh0,
-                                   void *stream);
+int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
+                                   int64_t g_st, const void *x, int64_t x_sb, int64_t x_st, const void *lens,
+                                   int32_t wide_lens, const float *carry, const void *dh, int64_t dh_sb, int64_t dh_st,
+                                   const float *dlast, void *dg, int64_t dg_sb, int64_t dg_st, void *dx, int64_t dx_sb,
+                                   int64_t dx_st, float *dh0, void *stream);
 /* One step for each of N rows: last = f state + (1 - f) x (32 bits; last may be state), h the same
  * rounded to `dtype`; g, x, h rows ldg, ldx, ldh elements apart, state and last contiguous. */
 int32_t parpy_b200_gated_step(int32_t dtype, int64_t N, int64_t D, const void *g, int64_t ldg, const void *x,

@@ -102,7 +102,20 @@ def _stage_arguments(spec, args, opts):
     if len(args) != len(spec.params):
         raise TypeError(f"{spec.name}() takes {len(spec.params)} positional arguments "
                         f"({', '.join(spec.params)}) but {len(args)} were given")
+    import torch
+    from .buffer import _torch_dtypes
+    device = torch.cuda.current_device() if torch.cuda.is_initialized() else None     # a host tensor says -1
+    types, strided = _torch_dtypes(), torch.strided
     for i, (name, arg) in enumerate(zip(spec.params, args)):
+        if type(arg) is torch.Tensor and arg.get_device() == device:
+            # an array that CudaBuffer would wrap as it is needs no wrapping
+            if arg.dtype in types and not arg.requires_grad and arg.layout is strided and \
+                    (arg.is_contiguous() or str(spec.roles.get(name)).endswith("_rows")):
+                out.append(arg)
+                continue
+        elif arg is None or type(arg) is int or type(arg) is float:
+            out.append(arg)
+            continue
         if isinstance(arg, dict):
             d = {}
             for k, v in arg.items():

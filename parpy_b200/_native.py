@@ -80,10 +80,11 @@ SIGNATURES = {
                                         c_i32, c_ptr, c_ptr, c_ptr, c_ptr]),
     "parpy_b200_distill_topk_grad": (c_i32, [c_ptr, c_i32, c_i64, c_i64, c_i64, c_ptr, c_i32, c_ptr, c_i32, c_i64,
                                              c_f64, c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
-    "parpy_b200_gated_scan": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32,
-                                      c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
-    "parpy_b200_gated_scan_grad": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i32, c_ptr,
-                                           c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "parpy_b200_gated_scan": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr,
+                                      c_ptr, c_i32, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
+    "parpy_b200_gated_scan_grad": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64, c_ptr,
+                                           c_i32, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64,
+                                           c_i64, c_ptr, c_ptr]),
     "parpy_b200_gated_step": (c_i32, [c_i32, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr,
                                       c_ptr]),
 }

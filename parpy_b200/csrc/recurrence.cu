@@ -576,27 +576,24 @@ int32_t run_step(const void *g, const void *x, const float *state, void *h, floa
     return PB_OK;
 }
 
-Walk walk(const void *p, const int64_t *strides) {
-    return Walk{const_cast<void *>(p), strides ? strides[0] : 0, strides ? strides[1] : 0};
-}
+Walk walk(const void *p, int64_t sb, int64_t st) { return Walk{const_cast<void *>(p), sb, st}; }
 
 }  // namespace
 
 extern "C" {
 
-int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, const int64_t *g_strides,
-                              const void *x, const int64_t *x_strides, const float *h0, const void *lens,
-                              int32_t wide_lens, void *h, const int64_t *h_strides, float *last, float *carry,
-                              void *stream) {
+int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
+                              int64_t g_st, const void *x, int64_t x_sb, int64_t x_st, const float *h0,
+                              const void *lens, int32_t wide_lens, void *h, int64_t h_sb, int64_t h_st, float *last,
+                              float *carry, void *stream) {
     const char *what = "gated_scan";
     int32_t rc = check_scan(what, dtype, B, T, D);
     if (rc || B == 0 || D == 0) return rc;
-    PB_REQUIRE(T == 0 || (g_strides && x_strides && h_strides), "%s: null pointer (strides)", what);
     ScanArgs a = {};
     if (T > 0) {
-        a.g = walk(g, g_strides);
-        a.x = walk(x, x_strides);
-        a.h = walk(h, h_strides);
+        a.g = walk(g, g_sb, g_st);
+        a.x = walk(x, x_sb, x_st);
+        a.h = walk(h, h_sb, h_st);
         rc = check_walk(what, "g", a.g, dtype, B, T, D, false);
         if (!rc) rc = check_walk(what, "x", a.x, dtype, B, T, D, false);
         if (!rc) rc = check_walk(what, "h", a.h, dtype, B, T, D, true);
@@ -621,23 +618,22 @@ int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, co
     return vec ? run_forward<__half, true>(a, dev, s) : run_forward<__half, false>(a, dev, s);
 }
 
-int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g,
-                                   const int64_t *g_strides, const void *x, const int64_t *x_strides, const void *lens,
-                                   int32_t wide_lens, const float *carry, const void *dh, const int64_t *dh_strides,
-                                   const float *dlast, void *dg, const int64_t *dg_strides, void *dx,
-                                   const int64_t *dx_strides, float *dh0, void *stream) {
+int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
+                                   int64_t g_st, const void *x, int64_t x_sb, int64_t x_st, const void *lens,
+                                   int32_t wide_lens, const float *carry, const void *dh, int64_t dh_sb, int64_t dh_st,
+                                   const float *dlast, void *dg, int64_t dg_sb, int64_t dg_st, void *dx, int64_t dx_sb,
+                                   int64_t dx_st, float *dh0, void *stream) {
     const char *what = "gated_scan_grad";
     int32_t rc = check_scan(what, dtype, B, T, D);
     if (rc || B == 0 || D == 0) return rc;
     ScanArgs a = {};
     if (T > 0) {
-        PB_REQUIRE(g_strides && x_strides && dg_strides && dx_strides && carry && (!dh || dh_strides),
-                   "%s: null pointer (strides or carry)", what);
-        a.g = walk(g, g_strides);
-        a.x = walk(x, x_strides);
-        a.dh = walk(dh, dh_strides);
-        a.dg = walk(dg, dg_strides);
-        a.dx = walk(dx, dx_strides);
+        PB_REQUIRE(carry, "%s: null pointer (carry)", what);
+        a.g = walk(g, g_sb, g_st);
+        a.x = walk(x, x_sb, x_st);
+        a.dh = walk(dh, dh_sb, dh_st);
+        a.dg = walk(dg, dg_sb, dg_st);
+        a.dx = walk(dx, dx_sb, dx_st);
         rc = check_walk(what, "g", a.g, dtype, B, T, D, false);
         if (!rc) rc = check_walk(what, "x", a.x, dtype, B, T, D, false);
         if (!rc && dh) rc = check_walk(what, "dh", a.dh, dtype, B, T, D, false);

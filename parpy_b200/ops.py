@@ -62,13 +62,14 @@ def scalar(v, what):
     """Python value of an int/float argument or of a 0-d buffer. A device-resident
     0-d tensor costs one D2H read, remembered for as long as that tensor object
     lives and is not written to (its version counter is unchanged)."""
-    import weakref
     if isinstance(v, (bool, int, float)):
         return v
-    if isinstance(v, Buffer):
+    import weakref
+    import torch
+    if isinstance(v, (Buffer, torch.Tensor)):
         if len(v.shape) != 0:
-            raise TypeError(f"{what}: expected a scalar, got a buffer of shape {v.shape}")
-        t = v.buf
+            raise TypeError(f"{what}: expected a scalar, got a buffer of shape {tuple(v.shape)}")
+        t = v.buf if isinstance(v, Buffer) else v
         version = getattr(t, "_version", None)
         hit = _scalar_cache.get(id(t))
         if hit is not None and hit[0]() is t and hit[1] == version and version is not None:
@@ -85,12 +86,18 @@ def scalar(v, what):
     raise TypeError(f"{what}: expected an int, float or 0-d array, got {type(v)}")
 
 
-def given(v, what, shape, dtype, allow_none=False):
-    """The CUDA tensor behind an argument of exactly this shape, or None for None where that is allowed."""
-    t = tensor(v, what, dtype, len(shape), allow_none)
-    if t is not None and tuple(t.shape) != shape:
-        raise RuntimeError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
-    return t
+def given(fun, name, v, shape, dtypes, allow_none=False):
+    """The CUDA tensor behind an argument of exactly this shape and one of these types, or None for None where that
+    is allowed."""
+    if v is None and allow_none:
+        return None
+    if not isinstance(v, Buffer) and getattr(v, "shape", None) == shape and v.dtype in dtypes:
+        return v        # staged as it is: on the current device
+    what = f"{fun}: {name}"
+    t = tensor(v, what, dtypes, len(shape))
+    if tuple(t.shape) == shape:
+        return t
+    raise RuntimeError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
 
 
 def tensor(v, what, dtype=None, ndim=None, allow_none=False):
@@ -99,11 +106,11 @@ def tensor(v, what, dtype=None, ndim=None, allow_none=False):
         if allow_none:
             return None
         raise TypeError(f"{what}: missing array argument")
-    if not isinstance(v, Buffer):
+    import torch
+    if not isinstance(v, (Buffer, torch.Tensor)):
         raise TypeError(f"{what}: expected an array, got {type(v)}")
-    t = v.buf
+    t = v.buf if isinstance(v, Buffer) else v
     if t.is_cuda:
-        import torch
         if t.device.index != torch.cuda.current_device():
             raise RuntimeError(f"{what}: array lives on cuda:{t.device.index} but the current device is "
                                f"cuda:{torch.cuda.current_device()}")
@@ -121,26 +128,45 @@ def ptr(t):
 
 
 def current_stream():
+    return ctypes.c_void_p(_stream())
+
+
+def _types():
+    """torch types by what the kernels below take them for."""
+    if not _type_sets:
+        import torch
+        codes = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+        _type_sets.extend((codes, tuple(codes), (torch.float32,), (torch.int64, torch.int32), torch.int64))
+    return _type_sets
+
+
+_type_sets = []   # float type -> code of the C ABI, float types, float32, index types, int64
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream():
+    """The raw handle of torch's current stream on the current device."""
     import torch
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
-def _float_types():
-    import torch
-    return {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
-
-
-def _pitch(t, what, output=False):
+def _pitch(fun, name, t, output=False):
     """Strides of every dimension but the last of an array that is contiguous along its last."""
-    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}: the last dimension must be contiguous, got strides {t.stride()}")
+    strides = t.stride()
+    if t.is_contiguous():
+        return strides[:-1]
+    if t.numel() and t.shape[-1] > 1 and strides[-1] != 1:
+        raise ValueError(f"{fun}: {name}: the last dimension must be contiguous, got strides {strides}")
     if output:
         reach = t.shape[-1]
-        for n, s in sorted(zip(t.shape[:-1], t.stride()[:-1]), key=lambda d: d[1]):
+        for n, s in sorted(zip(t.shape[:-1], strides[:-1]), key=lambda d: d[1]):
             if n > 1 and s < reach:
-                raise ValueError(f"{what}: rows of an output must not overlap, got strides {t.stride()}")
-            reach = max(reach, s * (n - 1) + reach)
-    return tuple(t.stride()[:-1])
+                raise ValueError(f"{fun}: {name}: rows of an output must not overlap, got strides {strides}")
+            reach += s * (n - 1)
+    return strides[:-1]
 
 
 # ---- HMM forward ---------------------------------------------------------------
@@ -414,15 +440,13 @@ register(OpSpec("spmm_cell", ("A", "B", "C"),
 
 
 # ---- rows of vocabulary logits -------------------------------------------------------------------
-def _logits(fun, x, N, M, what="x", like=None, output=False):
-    """(tensor, dtype code, row pitch, N, M) of a matrix of logits."""
-    n, m = int(scalar(N, "N")), int(scalar(M, "M"))
-    types = _float_types()
-    t = given(x, f"{fun}: {what}", (n, m), like.dtype if like is not None else tuple(types))
+def _logits(fun, x, n, m, types, name="x", output=False):
+    """(tensor, row pitch) of a matrix of logits."""
+    t = given(fun, name, x, (n, m), types)
     if m < 1:
         raise RuntimeError(f"{fun}: needs at least one column, got M={m}")
-    (pitch,) = _pitch(t, f"{fun}: {what}", output)
-    return t, types[t.dtype], max(pitch, m) if n <= 1 else pitch, n, m
+    pitch = _pitch(fun, name, t, output)[0]
+    return t, pitch if n > 1 else max(pitch, m)
 
 
 def _temperature(fun, temperature):
@@ -432,42 +456,43 @@ def _temperature(fun, temperature):
     return t
 
 
-def _wide(t):
-    import torch
-    return int(t is not None and t.dtype == torch.int64)
-
-
 def _token_logprobs_call(opts, x, tokens, N, M, K, temperature, logp, lse, entropy, top_logp, top_index):
-    import torch
-    f, f32, whole = "token_logprobs", torch.float32, (torch.int64, torch.int32)
-    xt, dtype, ld, n, m = _logits(f, x, N, M)
-    k = int(scalar(K, "K"))
+    f = "token_logprobs"
+    codes, floats, f32, whole, i64 = _types()
+    n, m, k = int(scalar(N, "N")), int(scalar(M, "M")), int(scalar(K, "K"))
+    xt, ld = _logits(f, x, n, m, floats)
     if not 0 <= k <= min(m, _native.TOP_MAX):
         raise RuntimeError(f"{f}: K={k} is outside [0, {min(m, _native.TOP_MAX)}]")
-    tok = given(tokens, f"{f}: tokens", (n,), whole, allow_none=logp is None)
-    lp = given(logp, f"{f}: logp", (n,), f32, allow_none=True)
-    ls = given(lse, f"{f}: lse", (n,), f32)
-    en = given(entropy, f"{f}: entropy", (n,), f32, allow_none=True)
-    tl = given(top_logp, f"{f}: top_logp", (n, k), f32) if k else None
-    ti = given(top_index, f"{f}: top_index", (n, k), whole) if k else None
+    rows = (n,)
+    tok = given(f, "tokens", tokens, rows, whole, logp is None)
+    lp = given(f, "logp", logp, rows, f32, True)
+    ls = given(f, "lse", lse, rows, f32)
+    en = given(f, "entropy", entropy, rows, f32, True)
+    tl = given(f, "top_logp", top_logp, (n, k), f32) if k else None
+    ti = given(f, "top_index", top_index, (n, k), whole) if k else None
+    temp = _temperature(f, temperature)
     _native.check(_native.lib().parpy_b200_token_logprobs(
-        ptr(xt), dtype, ld, n, m, ptr(tok), _wide(tok), _temperature(f, temperature), k, ptr(lp), ptr(ls), ptr(en),
-        ptr(tl), ptr(ti), _wide(ti), current_stream()), f)
+        xt.data_ptr(), codes[xt.dtype], ld, n, m, _address(tok), tok is not None and tok.dtype == i64, temp, k,
+        _address(lp), ls.data_ptr(), _address(en), _address(tl), _address(ti), ti is not None and ti.dtype == i64,
+        _stream()), f)
 
 
 def _token_logprobs_grad_call(opts, x, tokens, N, M, temperature, lse, entropy, dlogp, dentropy, dx):
-    import torch
-    f, f32, whole = "token_logprobs_grad", torch.float32, (torch.int64, torch.int32)
-    xt, dtype, ld, n, m = _logits(f, x, N, M)
-    dt, _, ldd, _, _ = _logits(f, dx, N, M, "dx", like=xt, output=True)
-    tok = given(tokens, f"{f}: tokens", (n,), whole, allow_none=dlogp is None)
-    ls = given(lse, f"{f}: lse", (n,), f32)
-    dl = given(dlogp, f"{f}: dlogp", (n,), f32, allow_none=True)
-    de = given(dentropy, f"{f}: dentropy", (n,), f32, allow_none=True)
-    en = given(entropy, f"{f}: entropy", (n,), f32, allow_none=de is None)
+    f = "token_logprobs_grad"
+    codes, floats, f32, whole, i64 = _types()
+    n, m = int(scalar(N, "N")), int(scalar(M, "M"))
+    xt, ld = _logits(f, x, n, m, floats)
+    dt, ldd = _logits(f, dx, n, m, (xt.dtype,), "dx", True)
+    rows = (n,)
+    tok = given(f, "tokens", tokens, rows, whole, dlogp is None)
+    ls = given(f, "lse", lse, rows, f32)
+    dl = given(f, "dlogp", dlogp, rows, f32, True)
+    de = given(f, "dentropy", dentropy, rows, f32, True)
+    en = given(f, "entropy", entropy, rows, f32, de is None)
+    temp = _temperature(f, temperature)
     _native.check(_native.lib().parpy_b200_token_logprobs_grad(
-        ptr(xt), dtype, ld, n, m, ptr(tok), _wide(tok), _temperature(f, temperature), ptr(ls), ptr(en), ptr(dl),
-        ptr(de), ptr(dt), ldd, current_stream()), f)
+        xt.data_ptr(), codes[xt.dtype], ld, n, m, _address(tok), tok is not None and tok.dtype == i64, temp,
+        ls.data_ptr(), _address(en), _address(dl), _address(de), dt.data_ptr(), ldd, _stream()), f)
 
 
 register(OpSpec("token_logprobs",
@@ -479,43 +504,46 @@ register(OpSpec("token_logprobs_grad",
                 {"x": "in_rows", "dx": "out_rows"}, _token_logprobs_grad_call, doc="gradient of token_logprobs"))
 
 
-def _teacher(f, index, values, n, K):
-    import torch
+def _teacher(f, index, values, n, K, floats, whole):
     k = int(scalar(K, "K"))
     if not 1 <= k <= _native.LIST_MAX:
         raise RuntimeError(f"{f}: K={k} is outside [1, {_native.LIST_MAX}]")
-    it = given(index, f"{f}: index", (n, k), (torch.int64, torch.int32))
-    vt = given(values, f"{f}: values", (n, k), tuple(_float_types()))
-    return it, vt, _float_types()[vt.dtype], k
+    return given(f, "index", index, (n, k), whole), given(f, "values", values, (n, k), floats), k
 
 
 def _distill_topk_call(opts, x, index, values, N, M, K, temperature, tail, loss, lse, rest):
-    import torch
-    f, f32 = "distill_topk", torch.float32
-    xt, dtype, ld, n, m = _logits(f, x, N, M)
-    it, vt, vtype, k = _teacher(f, index, values, n, K)
+    f = "distill_topk"
+    codes, floats, f32, whole, i64 = _types()
+    n, m = int(scalar(N, "N")), int(scalar(M, "M"))
+    xt, ld = _logits(f, x, n, m, floats)
+    it, vt, k = _teacher(f, index, values, n, K, floats, whole)
     bucket = int(bool(scalar(tail, "tail")))
-    lo = given(loss, f"{f}: loss", (n,), f32)
-    ls = given(lse, f"{f}: lse", (n,), f32)
-    re = given(rest, f"{f}: rest", (n,), f32, allow_none=not bucket)
+    rows = (n,)
+    lo = given(f, "loss", loss, rows, f32)
+    ls = given(f, "lse", lse, rows, f32)
+    re = given(f, "rest", rest, rows, f32, not bucket)
+    temp = _temperature(f, temperature)
     _native.check(_native.lib().parpy_b200_distill_topk(
-        ptr(xt), dtype, ld, n, m, ptr(it), _wide(it), ptr(vt), vtype, k, _temperature(f, temperature), bucket, ptr(lo),
-        ptr(ls), ptr(re), current_stream()), f)
+        xt.data_ptr(), codes[xt.dtype], ld, n, m, it.data_ptr(), it.dtype == i64, vt.data_ptr(), codes[vt.dtype], k,
+        temp, bucket, lo.data_ptr(), ls.data_ptr(), _address(re), _stream()), f)
 
 
 def _distill_topk_grad_call(opts, x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
-    import torch
-    f, f32 = "distill_topk_grad", torch.float32
-    xt, dtype, ld, n, m = _logits(f, x, N, M)
-    dt, _, ldd, _, _ = _logits(f, dx, N, M, "dx", like=xt, output=True)
-    it, vt, vtype, k = _teacher(f, index, values, n, K)
+    f = "distill_topk_grad"
+    codes, floats, f32, whole, i64 = _types()
+    n, m = int(scalar(N, "N")), int(scalar(M, "M"))
+    xt, ld = _logits(f, x, n, m, floats)
+    dt, ldd = _logits(f, dx, n, m, (xt.dtype,), "dx", True)
+    it, vt, k = _teacher(f, index, values, n, K, floats, whole)
     bucket = int(bool(scalar(tail, "tail")))
-    ls = given(lse, f"{f}: lse", (n,), f32)
-    re = given(rest, f"{f}: rest", (n,), f32, allow_none=not bucket)
-    dl = given(dloss, f"{f}: dloss", (n,), f32)
+    rows = (n,)
+    ls = given(f, "lse", lse, rows, f32)
+    re = given(f, "rest", rest, rows, f32, not bucket)
+    dl = given(f, "dloss", dloss, rows, f32)
+    temp = _temperature(f, temperature)
     _native.check(_native.lib().parpy_b200_distill_topk_grad(
-        ptr(xt), dtype, ld, n, m, ptr(it), _wide(it), ptr(vt), vtype, k, _temperature(f, temperature), bucket, ptr(ls),
-        ptr(re), ptr(dl), ptr(dt), ldd, current_stream()), f)
+        xt.data_ptr(), codes[xt.dtype], ld, n, m, it.data_ptr(), it.dtype == i64, vt.data_ptr(), codes[vt.dtype], k,
+        temp, bucket, ls.data_ptr(), _address(re), dl.data_ptr(), dt.data_ptr(), ldd, _stream()), f)
 
 
 register(OpSpec("distill_topk",
@@ -528,68 +556,67 @@ register(OpSpec("distill_topk_grad",
 
 
 # ---- gated linear recurrence ------------------------------------------------------------------------
-def _steps(f, name, a, shape, like=None, output=False, allow_none=False):
-    """(tensor, its two strides as a host array) of one [B, T, D] argument."""
-    t = given(a, f"{f}: {name}", shape, like.dtype if like is not None else tuple(_float_types()), allow_none)
-    if t is None:
-        return None, None
-    return t, (ctypes.c_int64 * 2)(*_pitch(t, f"{f}: {name}", output))
-
-
-def _scan_shape(f, B, T, D):
-    b, t, d = (int(scalar(v, n)) for v, n in ((B, "B"), (T, "T"), (D, "D")))
-    if min(b, t, d) < 0:
-        raise RuntimeError(f"{f}: negative shape {(b, t, d)}")
-    return b, t, d
-
-
 def _gated_scan_call(opts, g, x, h0, lens, B, T, D, h, last, carry):
-    import torch
-    f, f32 = "gated_scan", torch.float32
-    b, t, d = _scan_shape(f, B, T, D)
-    gt, gs = _steps(f, "g", g, (b, t, d))
-    xt, xs = _steps(f, "x", x, (b, t, d), gt)
-    ht, hs = _steps(f, "h", h, (b, t, d), gt, output=True)
-    first = given(h0, f"{f}: h0", (b, d), f32, allow_none=True)
-    n = given(lens, f"{f}: lens", (b,), (torch.int64, torch.int32), allow_none=True)
-    end = given(last, f"{f}: last", (b, d), f32, allow_none=True)
-    kept = given(carry, f"{f}: carry", (b, -(-t // _native.SCAN_TILE), d), f32, allow_none=True)
+    f = "gated_scan"
+    codes, floats, f32, whole, i64 = _types()
+    b, t, d = int(scalar(B, "B")), int(scalar(T, "T")), int(scalar(D, "D"))
+    if b < 0 or t < 0 or d < 0:
+        raise RuntimeError(f"{f}: negative shape {(b, t, d)}")
+    steps, states = (b, t, d), (b, d)
+    gt = given(f, "g", g, steps, floats)
+    same = (gt.dtype,)
+    xt = given(f, "x", x, steps, same)
+    ht = given(f, "h", h, steps, same)
+    first = given(f, "h0", h0, states, f32, True)
+    n = given(f, "lens", lens, (b,), whole, True)
+    end = given(f, "last", last, states, f32, True)
+    kept = given(f, "carry", carry, (b, -(-t // _native.SCAN_TILE), d), f32, True)
     _native.check(_native.lib().parpy_b200_gated_scan(
-        _float_types()[gt.dtype], b, t, d, ptr(gt), gs, ptr(xt), xs, ptr(first), ptr(n), _wide(n), ptr(ht), hs,
-        ptr(end), ptr(kept), current_stream()), f)
+        codes[gt.dtype], b, t, d, gt.data_ptr(), *_pitch(f, "g", gt), xt.data_ptr(), *_pitch(f, "x", xt),
+        _address(first), _address(n), n is not None and n.dtype == i64, ht.data_ptr(), *_pitch(f, "h", ht, True),
+        _address(end), _address(kept), _stream()), f)
 
 
 def _gated_scan_grad_call(opts, g, x, lens, B, T, D, carry, dh, dlast, dg, dx, dh0):
-    import torch
-    f, f32 = "gated_scan_grad", torch.float32
-    b, t, d = _scan_shape(f, B, T, D)
-    gt, gs = _steps(f, "g", g, (b, t, d))
-    xt, xs = _steps(f, "x", x, (b, t, d), gt)
-    dt, ds = _steps(f, "dh", dh, (b, t, d), gt, allow_none=True)
-    dgt, dgs = _steps(f, "dg", dg, (b, t, d), gt, output=True)
-    dxt, dxs = _steps(f, "dx", dx, (b, t, d), gt, output=True)
-    n = given(lens, f"{f}: lens", (b,), (torch.int64, torch.int32), allow_none=True)
-    kept = given(carry, f"{f}: carry", (b, -(-t // _native.SCAN_TILE), d), f32)
-    end = given(dlast, f"{f}: dlast", (b, d), f32, allow_none=True)
-    first = given(dh0, f"{f}: dh0", (b, d), f32, allow_none=True)
+    f = "gated_scan_grad"
+    codes, floats, f32, whole, i64 = _types()
+    b, t, d = int(scalar(B, "B")), int(scalar(T, "T")), int(scalar(D, "D"))
+    if b < 0 or t < 0 or d < 0:
+        raise RuntimeError(f"{f}: negative shape {(b, t, d)}")
+    steps, states = (b, t, d), (b, d)
+    gt = given(f, "g", g, steps, floats)
+    same = (gt.dtype,)
+    xt = given(f, "x", x, steps, same)
+    dt = given(f, "dh", dh, steps, same, True)
+    dgt = given(f, "dg", dg, steps, same)
+    dxt = given(f, "dx", dx, steps, same)
+    n = given(f, "lens", lens, (b,), whole, True)
+    kept = given(f, "carry", carry, (b, -(-t // _native.SCAN_TILE), d), f32)
+    end = given(f, "dlast", dlast, states, f32, True)
+    first = given(f, "dh0", dh0, states, f32, True)
     _native.check(_native.lib().parpy_b200_gated_scan_grad(
-        _float_types()[gt.dtype], b, t, d, ptr(gt), gs, ptr(xt), xs, ptr(n), _wide(n), ptr(kept), ptr(dt), ds,
-        ptr(end), ptr(dgt), dgs, ptr(dxt), dxs, ptr(first), current_stream()), f)
+        codes[gt.dtype], b, t, d, gt.data_ptr(), *_pitch(f, "g", gt), xt.data_ptr(), *_pitch(f, "x", xt), _address(n),
+        n is not None and n.dtype == i64, kept.data_ptr(), _address(dt), *(_pitch(f, "dh", dt) if dt is not None else (0, 0)),
+        _address(end), dgt.data_ptr(), *_pitch(f, "dg", dgt, True), dxt.data_ptr(), *_pitch(f, "dx", dxt, True),
+        _address(first), _stream()), f)
 
 
 def _gated_step_call(opts, g, x, state, N, D, h, last):
-    import torch
-    f, f32 = "gated_step", torch.float32
+    f = "gated_step"
+    codes, floats, f32, whole, i64 = _types()
     n, d = int(scalar(N, "N")), int(scalar(D, "D"))
-    gt = given(g, f"{f}: g", (n, d), tuple(_float_types()))
-    xt = given(x, f"{f}: x", (n, d), gt.dtype)
-    ht = given(h, f"{f}: h", (n, d), gt.dtype)
-    before = given(state, f"{f}: state", (n, d), f32)
-    after = given(last, f"{f}: last", (n, d), f32)
-    (lg,), (lx,), (lh,) = (_pitch(a, f"{f}: {w}", w == "h") for a, w in ((gt, "g"), (xt, "x"), (ht, "h")))
+    if n < 0 or d < 0:
+        raise RuntimeError(f"{f}: negative shape {(n, d)}")
+    rows = (n, d)
+    gt = given(f, "g", g, rows, floats)
+    same = (gt.dtype,)
+    xt = given(f, "x", x, rows, same)
+    ht = given(f, "h", h, rows, same)
+    before = given(f, "state", state, rows, f32)
+    after = given(f, "last", last, rows, f32)
     _native.check(_native.lib().parpy_b200_gated_step(
-        _float_types()[gt.dtype], n, d, ptr(gt), lg, ptr(xt), lx, ptr(before), ptr(ht), lh, ptr(after),
-        current_stream()), f)
+        codes[gt.dtype], n, d, gt.data_ptr(), *_pitch(f, "g", gt), xt.data_ptr(), *_pitch(f, "x", xt),
+        before.data_ptr(), ht.data_ptr(), *_pitch(f, "h", ht, True), after.data_ptr(), _stream()), f)
 
 
 register(OpSpec("gated_scan", ("g", "x", "h0", "lens", "B", "T", "D", "h", "last", "carry"),

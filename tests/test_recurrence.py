@@ -432,19 +432,17 @@ def test_refusals():
 
 
 def test_native_entries_refuse_before_any_launch(native):
-    import ctypes
     lib = native.lib()
-    st = (ctypes.c_int64 * 2)(32, 8)
+    st = (32, 8)
 
     def scan(dtype=0, b=2, t=4, d=8, g=64, gs=st, h=64, hs=st):
-        return lib.parpy_b200_gated_scan(dtype, b, t, d, g, gs, 64, st, None, None, 1, h, hs, None, None, None)
+        return lib.parpy_b200_gated_scan(dtype, b, t, d, g, *gs, 64, *st, None, None, 1, h, *hs, None, None, None)
     for kw, match in ((dict(dtype=5), "element type"), (dict(b=-1), "shape"), (dict(g=None), "null"),
-                      (dict(gs=None), "null"), (dict(g=66), "misaligned"),
-                      (dict(hs=(ctypes.c_int64 * 2)(8, 8)), "overlap"), (dict(hs=(ctypes.c_int64 * 2)(24, 8)), "overlap"),
-                      (dict(gs=(ctypes.c_int64 * 2)(-8, 8)), "negative")):
+                      (dict(h=None), "null"), (dict(g=66), "misaligned"), (dict(hs=(8, 8)), "overlap"),
+                      (dict(hs=(24, 8)), "overlap"), (dict(gs=(-8, 8)), "negative")):
         assert scan(**kw) != 0 and match in native.error_message(), (kw, native.error_message())
-    assert lib.parpy_b200_gated_scan_grad(0, 2, 4, 8, 64, st, 64, st, None, 1, None, None, None, None, 64, st, 64, st,
-                                          None, None) != 0
+    assert lib.parpy_b200_gated_scan_grad(0, 2, 4, 8, 64, *st, 64, *st, None, 1, None, None, 0, 0, None, 64, *st, 64,
+                                          *st, None, None) != 0
     assert "carry" in native.error_message()
     assert lib.parpy_b200_gated_step(0, 2, 8, 64, 8, 64, 8, 64, 64, 4, 64, None) != 0
     assert "overlap" in native.error_message()
