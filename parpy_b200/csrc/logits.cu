@@ -260,8 +260,11 @@ struct List {
     int bad;
 };
 
+// Every thread of the CTA takes part. Second mentions are found by whole warps: an entry against the lanes' share of
+// the entries before it.
 template <typename T>
 __device__ void load_list(List &l, const RowArgs &a, long long row, const T *xr) {
+    const int lane = threadIdx.x & 31;
     if (threadIdx.x == 0) l.bad = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
@@ -273,11 +276,12 @@ __device__ void load_list(List &l, const RowArgs &a, long long row, const T *xr)
         l.x[k] = in ? Elem<T>::to_float(xr[i]) : 0.0f;
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
+    for (int k = threadIdx.x >> 5; k < a.K; k += blockDim.x >> 5) {
         const int c = l.col[k];
-        bool used = c >= 0;
-        for (int j = 0; j < k && used; ++j) used = l.col[j] != c;
-        l.used[k] = used;
+        bool seen = false;
+        for (int j = lane; j < k; j += 32) seen |= l.col[j] == c;
+        const bool again = __any_sync(0xffffffffu, seen);
+        if (lane == 0) l.used[k] = c >= 0 && !again;
     }
     __syncthreads();
 }
@@ -290,7 +294,8 @@ struct Teacher {
     int any;          // entries in use
 };
 
-__device__ Teacher warp_teacher(const List &l, int K, bool tail, double inv_t) {
+template <bool TAIL, bool STUDENT>
+__device__ Teacher warp_teacher(const List &l, int K, double inv_t) {
     const int lane = threadIdx.x & 31;
     float vm = -INFINITY, xm = -INFINITY;
     int n = 0;
@@ -300,27 +305,26 @@ __device__ Teacher warp_teacher(const List &l, int K, bool tail, double inv_t) {
             xm = fmaxf(xm, l.x[k]);
             ++n;
         }
-    vm = pb::warp_max(vm);
-    xm = pb::warp_max(xm);
+    if (!TAIL) vm = pb::warp_max(vm);
+    if (STUDENT) xm = pb::warp_max(xm);
     const float vref = isinf(vm) ? 0.0f : vm, xref = isinf(xm) ? 0.0f : xm;
     double sv = 0.0, sx = 0.0;
     for (int k = lane; k < K; k += 32)
         if (l.used[k]) {
-            sv += tail ? exp((double)l.v[k]) : (double)expf(l.v[k] - vref);
-            sx += (double)expf((float)(((double)l.x[k] - (double)xref) * inv_t));
+            sv += TAIL ? exp((double)l.v[k]) : (double)expf(l.v[k] - vref);
+            if (STUDENT) sx += (double)expf((float)(((double)l.x[k] - (double)xref) * inv_t));
         }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sv += __shfl_xor_sync(0xffffffffu, sv, o);
-        sx += __shfl_xor_sync(0xffffffffu, sx, o);
+        if (STUDENT) sx += __shfl_xor_sync(0xffffffffu, sx, o);
         n += __shfl_xor_sync(0xffffffffu, n, o);
     }
     Teacher t;
     t.any = n;
-    t.norm = tail ? 0.0f : (float)((double)vref + log(sv));
-    if (!tail && sv == 0.0) t.norm = 0.0f;        // no entry with mass: every q is exp(-inf) = 0
-    t.mass = !isfinite(sv) ? (double)NAN : tail ? sv : sv == 0.0 ? 0.0 : 1.0;
-    t.listed = sx == 0.0 ? -INFINITY : (double)xref * inv_t + log(sx);
+    t.norm = TAIL || sv == 0.0 ? 0.0f : vref + (float)log(sv);    // no entry with mass: every q is exp(-inf) = 0
+    t.mass = !isfinite(sv) ? (double)NAN : TAIL ? sv : sv == 0.0 ? 0.0 : 1.0;
+    t.listed = !STUDENT || sx == 0.0 ? -INFINITY : (double)xref * inv_t + log(sx);
     return t;
 }
 
@@ -358,7 +362,8 @@ struct ListSmem<THREADS, kRenorm> {
 template <int THREADS>
 struct ListSmem<THREADS, kTail> {
     List l;
-    int next[THREADS];
+    int head[THREADS];          // a thread's listed columns as a chain: first entry, -1 for none
+    short link[kListMax];       // the entry after this one
 };
 
 __device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
@@ -404,16 +409,17 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
     }
     int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
     if constexpr (LIST != kNone) {
-        if constexpr (LIST == kTail) s_list.next[tid] = INT_MAX;
+        if constexpr (LIST == kTail) s_list.head[tid] = -1;
         load_list(s_list.l, a, row, xr);
         if constexpr (LIST == kTail) {
             for (int k = tid; k < a.K; k += THREADS)
                 if (s_list.l.used[k]) {
-                    const int v = (int)(((long long)s_list.l.col[k] + rv.mis) / VE), owner = v % total;
-                    if (owner / THREADS == rank) atomicMin(&s_list.next[owner % THREADS], v);
+                    const int owner = ((s_list.l.col[k] + rv.mis) / VE) % total;
+                    if (owner / THREADS == rank)
+                        s_list.link[k] = (short)atomicExch(&s_list.head[owner % THREADS], k);
                 }
             __syncthreads();
-            next = s_list.next[tid];
+            for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) next = min(next, (s_list.l.col[k] + rv.mis) / VE);
         }
     }
 
@@ -427,21 +433,17 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
             if (v == next) {         // listed columns are summed apart: read as masked here
                 T *e = reinterpret_cast<T *>(&r);
                 const unsigned fill = Elem<T>::kFill;
-                int after = INT_MAX;
-                for (int k = 0; k < a.K; ++k)
-                    if (s_list.l.used[k]) {
-                        const long long at = (long long)s_list.l.col[k] + rv.mis;
-                        const int w = (int)(at / VE);
-                        if (w == v) {
-                            const int slot = (int)(at - (long long)v * VE);
+                next = INT_MAX;
+                for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) {
+                    const int at = s_list.l.col[k] + rv.mis, w = at / VE;
+                    if (w == v) {
 #pragma unroll
-                            for (int i = 0; i < VE; ++i)
-                                if (i == slot) e[i] = *reinterpret_cast<const T *>(&fill);
-                        } else if (w > v && w < after && w % total == me) {
-                            after = w;
-                        }
+                        for (int i = 0; i < VE; ++i)
+                            if (i == at % VE) e[i] = *reinterpret_cast<const T *>(&fill);
+                    } else if (w > v) {
+                        next = min(next, w);
                     }
-                next = after;
+                }
             }
         }
         const float vm = Elem<T>::vmax(r);
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
         const double S = (double)w.S;
         double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + log(S);
         if constexpr (LIST != kNone) {
-            const Teacher t = warp_teacher(s_list.l, a.K, LIST == kTail, a.inv_t);
+            const Teacher t = warp_teacher<LIST == kTail, LIST == kTail>(s_list.l, a.K, a.inv_t);
             const double rest = lse;
             if (LIST == kTail) lse = log_add(rest, t.listed);
             double loss = 0.0;
@@ -680,8 +682,7 @@ struct GradArgs {
 template <typename T, int THREADS, int LIST>
 __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int parts) {
     constexpr int VE = Elem<T>::VE, U = 4;
-    __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kTail> s_list;
-    __shared__ float s_fix[LIST == kNone ? 1 : kListMax];
+    __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kRenorm> s_list;
     __shared__ Teacher s_teacher;
     const RowArgs &a = g.r;
     const int tid = threadIdx.x;
@@ -694,12 +695,14 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
     const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15u) == 0;
     const float c = (float)(kLog2eD * a.inv_t);
 
-    // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the exceptions: the token's
-    // (gamma more) or the listed ones (their value from s_fix). ref is lse (or rest) in units of x, as a high and a
+    // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the token's
+    // (gamma more) and the listed ones (written last). ref is lse (or rest) in units of x, as a high and a
     // low part, because its rounding would scale the whole row.
     double base = (double)g.lse[row];
     float al = 0.0f, be = 0.0f, gamma = 0.0f;
-    int next = INT_MAX, slot = 0;             // the next vector of this thread that holds an exception
+    int tok_v = -1, tok_i = 0;                // vector and place of the token
+    double w = 0.0, W = 0.0, row_lse = base;
+    bool broken = false;
     const bool dead = base == -INFINITY;      // no finite logit in the row: no gradient
     if constexpr (LIST == kNone) {
         const long long token = a.tokens ? load_index(a.tokens, row, a.wide) : -1;
@@ -710,45 +713,32 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
             be = (float)(-de * kLn2 * a.inv_t);
             gamma = (float)(dl * a.inv_t);
             if (token >= 0 && token < a.M) {
-                next = (int)((token + rv.mis) / VE);
-                slot = (int)((token + rv.mis) % VE);
+                tok_v = (int)((token + rv.mis) / VE);
+                tok_i = (int)((token + rv.mis) % VE);
             }
         }
         if (token >= a.M) al = NAN;
     } else {
-        s_list.next[tid] = INT_MAX;
         load_list(s_list.l, a, row, xr);
         if (tid < 32) {
-            const Teacher t = warp_teacher(s_list.l, a.K, LIST == kTail, a.inv_t);
+            const Teacher t = warp_teacher<LIST == kTail, false>(s_list.l, a.K, a.inv_t);
             if (tid == 0) s_teacher = t;
         }
-        for (int k = tid; k < a.K; k += THREADS)
-            if (s_list.l.used[k]) {
-                const int v = (int)(((long long)s_list.l.col[k] + rv.mis) / VE), owner = v % total;
-                if (owner / THREADS == part) atomicMin(&s_list.next[owner % THREADS], v);
-            }
         __syncthreads();
-        next = s_list.next[tid];
         const Teacher t = s_teacher;
-        const double w = (double)g.dloss[row] * a.inv_t, lse = base;
-        const double left = LIST == kTail ? left_of(t, a.M) : 0.0, W = t.mass + left;
-        if (!dead) {
-            if (LIST == kTail) {
-                // exp(z - rest) cannot overflow where it is used, however little the student has there
-                base = (double)g.rest[row];
-                al = base == -INFINITY ? 0.0f : (float)(w * (W * exp(base - lse) - left));
-            } else {
-                al = (float)(w * W);
-            }
+        const double left = LIST == kTail ? left_of(t, a.M) : 0.0;
+        w = (double)g.dloss[row] * a.inv_t;
+        W = t.mass + left;
+        broken = s_list.l.bad || isnan(t.mass) || isnan(row_lse);
+        if (broken) {
+            al = NAN;
+        } else if (!dead && LIST == kTail) {
+            // exp(z - rest) cannot overflow where it is used, however little the student has there
+            base = (double)g.rest[row];
+            al = base == -INFINITY ? 0.0f : (float)(w * (W * exp(base - row_lse) - left));
+        } else if (!dead) {
+            al = (float)(w * W);
         }
-        const bool broken = s_list.l.bad || isnan(t.mass) || isnan(lse);
-        if (broken) al = NAN;
-        for (int k = tid; k < a.K; k += THREADS) {
-            const double z = (double)s_list.l.x[k] * a.inv_t;
-            const float p = z == -INFINITY ? 0.0f : expf((float)(z - lse)), q = expf(s_list.l.v[k] - t.norm);
-            s_fix[k] = broken ? NAN : dead ? 0.0f : (float)(w * (W * (double)p - (double)q));
-        }
-        __syncthreads();
     }
     if (base == -INFINITY) base = 0.0;        // every x it meets is -inf: exp2(-inf) = 0
     base /= a.inv_t;
@@ -763,27 +753,11 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
             const float e = pb::ex2_approx(t);
             f[i] = LIST == kNone ? e * fmaf(be, fmaxf(t, -1e30f), al) : e * al;
         }
-        if (v == next) {
-            if constexpr (LIST == kNone) {
+        if constexpr (LIST == kNone) {
+            if (v == tok_v) {
 #pragma unroll
                 for (int i = 0; i < VE; ++i)
-                    if (i == slot) f[i] += gamma;
-            } else {
-                int after = INT_MAX;
-                for (int k = 0; k < a.K; ++k)
-                    if (s_list.l.used[k]) {
-                        const long long at = (long long)s_list.l.col[k] + rv.mis;
-                        const int w = (int)(at / VE);
-                        if (w == v) {
-                            const int s = (int)(at - (long long)v * VE);
-#pragma unroll
-                            for (int i = 0; i < VE; ++i)
-                                if (i == s) f[i] = s_fix[k];
-                        } else if (w > v && w < after && w % total == me) {
-                            after = w;
-                        }
-                    }
-                next = after;
+                    if (i == tok_i) f[i] += gamma;
             }
         }
         const int c0 = rv.first(v);
@@ -807,6 +781,18 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
             if (v + u * total < rv.v1) put(r[u], v + u * total, true);
     }
     if (rv.nvec > rv.v1 && (rv.nvec > 1 || !rv.v0) && me == rv.v1 % total) put(rv.edge(rv.v1), rv.v1, false);
+    if constexpr (LIST != kNone) {
+        // the listed columns of this part's vectors, over what the pass wrote there (each column is listed once)
+        __syncthreads();
+        const float norm = s_teacher.norm;
+        for (int k = tid; k < a.K; k += THREADS)
+            if (s_list.l.used[k] && ((s_list.l.col[k] + rv.mis) / VE) % total / THREADS == part) {
+                const double z = (double)s_list.l.x[k] * a.inv_t;
+                const float p = z == -INFINITY ? 0.0f : expf((float)(z - row_lse)), q = expf(s_list.l.v[k] - norm);
+                dr[s_list.l.col[k]] =
+                    Elem<T>::from_float(broken ? NAN : dead ? 0.0f : (float)(w * (W * (double)p - (double)q)));
+            }
+    }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------
