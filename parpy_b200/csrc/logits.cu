@@ -32,94 +32,91 @@ constexpr double kLn2 = 0.693147180559945309417;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr int kTopMax = 128;         // alternatives a row can ask for
 constexpr int kListMax = 1024;       // entries of a teacher's list
-constexpr int kCand = 2048;          // candidates of one selection round
-constexpr int kGroups = 128;         // thread groups whose best values give the selection threshold
+constexpr int kCand = 1024;          // candidates of one selection round
+constexpr int kSample = 256;         // of them, where there are more, that give the next round's bound
+constexpr int kGroups = 128;         // most thread groups whose best values give the first bound
 constexpr int kMaxCluster = 8;
 
 using u64 = unsigned long long;
 
-// ---- element types ----------------------------------------------------------------------------
+// ---- element types: 32 bytes of a row, the widest load there is ------------------------------------------
+struct Vec {
+    unsigned w[8];
+};
+
 template <typename T>
 struct Elem;
 template <>
 struct Elem<float> {
-    static constexpr int VE = 4;
+    static constexpr int VE = 8;
     static constexpr unsigned kFill = 0xff800000u;   // -inf
     __device__ static float to_float(float v) { return v; }
     __device__ static float from_float(float v) { return v; }
-    __device__ static void unpack(const uint4 &r, float (&v)[4]) {
-        v[0] = __uint_as_float(r.x);
-        v[1] = __uint_as_float(r.y);
-        v[2] = __uint_as_float(r.z);
-        v[3] = __uint_as_float(r.w);
+    // elements 2 i and 2 i + 1
+    __device__ static void pair(const Vec &r, int i, float &a, float &b) {
+        a = __uint_as_float(r.w[2 * i]);
+        b = __uint_as_float(r.w[2 * i + 1]);
     }
-    __device__ static uint4 pack(const float (&v)[4]) {
-        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    __device__ static void set_pair(Vec &r, int i, float a, float b) {
+        r.w[2 * i] = __float_as_uint(a);
+        r.w[2 * i + 1] = __float_as_uint(b);
     }
-    __device__ static float vmax(const uint4 &r) {
-        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
-                     fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    __device__ static float vmax(const Vec &r) {
+        float m = __uint_as_float(r.w[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(r.w[i]));
+        return m;
     }
 };
 template <>
 struct Elem<__nv_bfloat16> {
-    static constexpr int VE = 8;
+    static constexpr int VE = 16;
     static constexpr unsigned kFill = 0xff80ff80u;
     __device__ static float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
     __device__ static __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-    __device__ static void unpack(const uint4 &r, float (&v)[8]) {
-        const unsigned w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+    __device__ static void pair(const Vec &r, int i, float &a, float &b) {
+        a = __uint_as_float(r.w[i] << 16);
+        b = __uint_as_float(r.w[i] & 0xffff0000u);
     }
-    __device__ static uint4 pack(const float (&v)[8]) {
-        unsigned w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const unsigned *>(&p);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+    __device__ static void set_pair(Vec &r, int i, float a, float b) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+        r.w[i] = *reinterpret_cast<const unsigned *>(&p);
     }
-    __device__ static float vmax(const uint4 &r) {
-        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&r);
-        const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    __device__ static float vmax(const Vec &r) {
+        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(r.w);
+        const __nv_bfloat162 m = __hmax2(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])),
+                                         __hmax2(__hmax2(p[4], p[5]), __hmax2(p[6], p[7])));
         return fmaxf(__low2float(m), __high2float(m));
     }
 };
 template <>
 struct Elem<__half> {
-    static constexpr int VE = 8;
+    static constexpr int VE = 16;
     static constexpr unsigned kFill = 0xfc00fc00u;
     __device__ static float to_float(__half v) { return __half2float(v); }
     __device__ static __half from_float(float v) { return __float2half_rn(v); }
-    __device__ static void unpack(const uint4 &r, float (&v)[8]) {
-        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(p[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
+    __device__ static void pair(const Vec &r, int i, float &a, float &b) {
+        const float2 f = __half22float2(reinterpret_cast<const __half2 *>(r.w)[i]);
+        a = f.x;
+        b = f.y;
     }
-    __device__ static uint4 pack(const float (&v)[8]) {
-        unsigned w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const unsigned *>(&p);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+    __device__ static void set_pair(Vec &r, int i, float a, float b) {
+        const __half2 p = __floats2half2_rn(a, b);
+        r.w[i] = *reinterpret_cast<const unsigned *>(&p);
     }
-    __device__ static float vmax(const uint4 &r) {
-        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
-        const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    __device__ static float vmax(const Vec &r) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(r.w);
+        const __half2 m = __hmax2(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])),
+                                  __hmax2(__hmax2(p[4], p[5]), __hmax2(p[6], p[7])));
         return fmaxf(__low2float(m), __high2float(m));
     }
 };
+template <typename T>
+__device__ __forceinline__ float element(const Vec &r, int i) {
+    float a, b;
+    Elem<T>::pair(r, i >> 1, a, b);
+    return i & 1 ? b : a;
+}
 
 // ---- packed fp32 pairs (two lanes of one 64-bit register, one instruction each) ------------------------
 __device__ __forceinline__ u64 pack2(float a, float b) {
@@ -146,9 +143,9 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
     return r;
 }
 
-// ---- a row as 16-byte vectors -----------------------------------------------------------------------------
+// ---- a row as 32-byte vectors -----------------------------------------------------------------------------
 // Vector v of a row holds the columns [v VE - mis, v VE - mis + VE), where mis is the number of elements between the
-// last 16-byte boundary and the row's start: rows may start at any element. Only the first and the last vector can
+// last 32-byte boundary and the row's start: rows may start at any element. Only the first and the last vector can
 // be partial; they are fetched element by element and filled up with -inf, so nothing outside the row is read.
 template <typename T>
 struct Row {
@@ -156,20 +153,21 @@ struct Row {
     int M, mis, nvec, v0, v1;   // vectors [v0, v1) are whole
     __device__ Row(const T *row, int m) : p(row), M(m) {
         constexpr int VE = Elem<T>::VE;
-        mis = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+        mis = (int)((reinterpret_cast<uintptr_t>(row) & 31u) / sizeof(T));
         nvec = (int)(((long long)M + mis + VE - 1) / VE);
         v0 = mis ? 1 : 0;
         v1 = (int)(((long long)M + mis) / VE);
     }
     __device__ bool whole(int v) const { return v >= v0 && v < v1; }
+    __device__ bool tail() const { return nvec > v1 && (nvec > 1 || !v0); }   // vector v1 is partial and not the first
     __device__ int first(int v) const { return v * Elem<T>::VE - mis; }
-    __device__ const uint4 *at(int v) const {
-        return reinterpret_cast<const uint4 *>(p + (long long)v * Elem<T>::VE - mis);
-    }
-    __device__ uint4 edge(int v) const {
+    __device__ const T *at(int v) const { return p + (long long)v * Elem<T>::VE - mis; }
+    __device__ Vec edge(int v) const {
         constexpr int VE = Elem<T>::VE;
-        uint4 r = make_uint4(Elem<T>::kFill, Elem<T>::kFill, Elem<T>::kFill, Elem<T>::kFill);
-        T *e = reinterpret_cast<T *>(&r);
+        Vec r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = Elem<T>::kFill;
+        T *e = reinterpret_cast<T *>(r.w);
         const int c0 = first(v);
 #pragma unroll
         for (int i = 0; i < VE; ++i)
@@ -178,12 +176,28 @@ struct Row {
     }
 };
 
-__device__ __forceinline__ uint4 ld_once(const uint4 *p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+// The forward pass may read through the non-coherent path; a gradient written over its own logits may not.
+__device__ __forceinline__ Vec ld_const(const void *p) {
+    Vec r;
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                   "=r"(r.w[7])
                  : "l"(p));
     return r;
+}
+__device__ __forceinline__ Vec ld_stream(const void *p) {
+    Vec r;
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                   "=r"(r.w[7])
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+__device__ __forceinline__ void st_stream(void *p, const Vec &r) {
+    asm volatile("st.global.cs.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+                 "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]), "l"(p)
+                 : "memory");
 }
 
 // ---- the order of (value, lowest column) as one 64-bit key: larger is better, 0 is "none" ------------------
@@ -370,10 +384,10 @@ __device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
-// One row per cluster of C CTAs (grid.x = rows x C); vectors dealt round robin to the cluster's threads.
+// Rows dealt to clusters of C CTAs, vectors of a row round robin to the cluster's threads.
 template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
-__global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(const RowArgs a, const int C) {
-    constexpr int VE = Elem<T>::VE, U = 4, NW = THREADS / 32, GL = THREADS / kGroups;
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowArgs a, const int C) {
+    constexpr int VE = Elem<T>::VE, NW = THREADS / 32, U = ENT ? 1 : 2;
     __shared__ Sums s_warp[NW];
     __shared__ Sums s_rank[kMaxCluster];
     __shared__ double s_ref, s_log;     // the row's reference value and log(S): lse = ref / temperature + log(S)
@@ -382,23 +396,40 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
-    const long long row = blockIdx.x / C;
+    const long long rows_apart = gridDim.x / C;
     const int total = C * THREADS, me = rank * THREADS + tid;
-    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
-    const Row<T> rv(xr, a.M);
     const float c = (float)(kLog2eD * a.inv_t);
     const float slack = 8.0f / c;
+    const int reach = (U - 1) * total;
+    Vec r0[U], r1[U];
+    auto load = [&](Vec (&r)[U], const Row<T> &rv, int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) r[u] = ld_const(rv.at(at + u * total));
+    };
+    auto open_row = [&](long long row) {     // a row's first vectors, before anything else of it
+        const Row<T> rv(static_cast<const T *>(a.x) + row * a.ldx, a.M);
+        const int v = me < rv.v0 ? me + total : me;
+        if (v + reach < rv.v1) load(r0, rv, v);
+    };
+    open_row(blockIdx.x / C);
 
     if constexpr (TOP) {
         if (C > 1 && rank == 0)
             for (int i = tid; i < C * a.K; i += THREADS) s_top.merge[i] = 0;
+    }
+    if (C > 1) cluster_arrive();     // matched before the first store into rank 0's shared memory
+
+  // with C > 1 every cluster has one row
+  for (long long row = blockIdx.x / C; row < a.N; row += rows_apart) {
+    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
+    const Row<T> rv(xr, a.M);
+    if constexpr (TOP) {
         if (tid == 0) {
             s_top.tau = 0;
             s_top.nsel = 0;
             s_top.ncand = 0;
         }
     }
-    if (C > 1) cluster_arrive();     // matched before the first store into rank 0's shared memory
     float x_token = 0.0f;
     long long token = -1;
     if constexpr (LIST == kNone) {
@@ -428,19 +459,20 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
     u64 S2 = 0, E2 = 0;
     const u64 c2 = pack2(c, c);
 
-    auto take = [&](uint4 r, int v) {
+    auto take = [&](const Vec &got, int at) {
+        Vec r = got;
         if constexpr (LIST == kTail) {
-            if (v == next) {         // listed columns are summed apart: read as masked here
-                T *e = reinterpret_cast<T *>(&r);
+            if (at == next) {         // listed columns are summed apart: read as masked here
+                T *e = reinterpret_cast<T *>(r.w);
                 const unsigned fill = Elem<T>::kFill;
                 next = INT_MAX;
                 for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) {
-                    const int at = s_list.l.col[k] + rv.mis, w = at / VE;
-                    if (w == v) {
+                    const int col = s_list.l.col[k] + rv.mis, w = col / VE;
+                    if (w == at) {
 #pragma unroll
                         for (int i = 0; i < VE; ++i)
-                            if (i == at % VE) e[i] = *reinterpret_cast<const T *>(&fill);
-                    } else if (w > v) {
+                            if (i == col % VE) e[i] = *reinterpret_cast<const T *>(&fill);
+                    } else if (w > at) {
                         next = min(next, w);
                     }
                 }
@@ -450,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
         if constexpr (TOP) {
             if (vm > best) {
                 best = vm;
-                best_v = v;
+                best_v = at;
             }
         }
         if (vm > lim) {
@@ -469,35 +501,59 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
             ref = vm;
             lim = vm + slack;
         }
-        float f[VE];
-        Elem<T>::unpack(r, f);
-        const u64 nref = pack2(-ref, -ref);
+        const u64 nref = pack2(-ref, -ref), before = E2;
 #pragma unroll
-        for (int i = 0; i < VE; i += 2) {
-            const u64 t = mul2(add2(pack2(f[i], f[i + 1]), nref), c2);
-            float t0, t1;
+        for (int i = 0; i < VE / 2; ++i) {
+            float x0, x1, t0, t1;
+            Elem<T>::pair(r, i, x0, x1);
+            const u64 t = mul2(add2(pack2(x0, x1), nref), c2);
             unpack2(t, t0, t1);
             const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
             S2 = add2(S2, e);
-            if constexpr (ENT) E2 = fma2(e, pack2(fmaxf(t0, -1e30f), fmaxf(t1, -1e30f)), E2);
+            if constexpr (ENT) E2 = fma2(e, t, E2);
+        }
+        if constexpr (ENT) {
+            // a masked column adds 0 times -inf: seen by the NaN it leaves, and added again with t kept finite
+            float e0, e1;
+            unpack2(E2, e0, e1);
+            if (isnan(e0 + e1)) {
+                E2 = before;
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    float x0, x1, t0, t1;
+                    Elem<T>::pair(r, i, x0, x1);
+                    unpack2(mul2(add2(pack2(x0, x1), nref), c2), t0, t1);
+                    const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
+                    E2 = fma2(e, pack2(fmaxf(t0, -1e30f), fmaxf(t1, -1e30f)), E2);
+                }
+            }
         }
     };
-
+    auto take_all = [&](const Vec (&r)[U], int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) take(r[u], at + u * total);
+    };
     if (rv.v0 && me == 0) take(rv.edge(0), 0);
-    {
-        // at most 2^29 + 1 vectors and 2^12 threads: no sum here leaves 32 bits
-        for (int v = me < rv.v0 ? me + total : me; v < rv.v1; v += U * total) {
-            uint4 r[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (v + u * total < rv.v1) r[u] = ld_once(rv.at(v + u * total));
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (v + u * total < rv.v1) take(r[u], v + u * total);
-        }
+    // at most 2^28 + 1 vectors and 2^12 threads: no sum of them leaves 32 bits
+    int v = me < rv.v0 ? me + total : me;
+    bool more = v + reach < rv.v1;
+    while (more) {                   // the next vectors are on their way while these are summed
+        int then = v + U * total;
+        more = then + reach < rv.v1;
+        if (more) load(r1, rv, then);
+        take_all(r0, v);
+        v = then;
+        if (!more) break;
+        then = v + U * total;
+        more = then + reach < rv.v1;
+        if (more) load(r0, rv, then);
+        take_all(r1, v);
+        v = then;
     }
-    if (rv.nvec > rv.v1 && (rv.nvec > 1 || !rv.v0) && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
+    for (; v < rv.v1; v += total) take(ld_const(rv.at(v)), v);
+    if (rv.tail() && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
 
+    if (row + rows_apart < a.N) open_row(row + rows_apart);
     Sums mine;
     {
         float s0, s1, e0, e1;
@@ -508,20 +564,20 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
     mine = warp_join<ENT>(mine, c);
     if (lane == 0) s_warp[warp] = mine;
 
-    u64 key = 0;
-    int sub = 0, group = 0;
-    u64 group_key = 0;
+    // A group's best value is one of the row's elements, so the K-th best of the groups' values bounds the K-th best
+    // element from below: only threads whose own best reaches it can hold one of the K. Few groups rank fast, many bound
+    // well: with 64 groups and K = 20 about 24 elements pass, with 128 about 22. A vector's place stands for its
+    // columns; the bound takes the vector's last column, so that it never cuts off a tie.
+    u64 key = 0, group_key = 0;
+    const int groups = a.K <= 32 ? kGroups / 2 : kGroups, GL = THREADS / groups, sub = tid & (GL - 1);
     if constexpr (TOP) {
         key = best_v < 0 ? 0 : key_of(best, max(rv.first(best_v), 0));
         group_key = key;
-#pragma unroll
-        for (int o = GL / 2; o > 0; o >>= 1) {
+        for (int o = GL >> 1; o > 0; o >>= 1) {
             const u64 other = __shfl_xor_sync(0xffffffffu, group_key, o);
             group_key = other > group_key ? other : group_key;
         }
-        sub = tid % GL;
-        group = tid / GL;
-        if (sub == 0) s_top.group[group] = group_key;
+        if (sub == 0) s_top.group[tid / GL] = group_key;
     }
     __syncthreads();
     if (warp == 0) {
@@ -533,46 +589,40 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
 
     int n_local = 0;
     if constexpr (TOP) {
-        // A group's best value is one of the row's elements, so the K-th best of the groups' values bounds the K-th
-        // best element from below: only threads whose own best reaches it can hold one of the K. A vector's
-        // place stands for its columns; the bound takes the vector's last column so that it never cuts off a tie.
         int above = 0;
-        for (int j = sub; j < kGroups; j += GL) above += s_top.group[j] > group_key;
-#pragma unroll
-        for (int o = GL / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        for (int j = sub; j < groups; j += GL) above += s_top.group[j] > group_key;
+        for (int o = GL >> 1; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
         if (sub == 0 && above == a.K - 1 && group_key != 0) s_top.tau = group_key - (VE - 1);
         __syncthreads();
         u64 tau = s_top.tau;
         if (key != 0 && key >= tau) s_top.sel[atomicAdd(&s_top.nsel, 1)] = tid;
         __syncthreads();
-        const int per = (rv.nvec + total - 1) / total;
-        const long long items = (long long)s_top.nsel * per;
+        const int nsel = s_top.nsel;
         while (true) {
-            for (long long it = tid; it < items; it += THREADS) {
-                const int s = s_top.sel[it / per];
-                const long long v = (long long)rank * THREADS + s + (it % per) * (long long)total;
-                if (v >= rv.nvec) continue;
-                const uint4 r = rv.whole((int)v) ? ld_once(rv.at((int)v)) : rv.edge((int)v);
-                float f[VE];
-                Elem<T>::unpack(r, f);
-                const int c0 = rv.first((int)v);
+            for (int i = warp; i < nsel; i += NW) {      // a warp goes through the vectors of one such thread
+                const int from = rank * THREADS + s_top.sel[i];
+                for (int at = from + lane * total; at < rv.nvec; at += 32 * total) {
+                    const Vec r = rv.whole(at) ? ld_const(rv.at(at)) : rv.edge(at);
+                    const int c0 = rv.first(at);
+                    if (order_of(Elem<T>::vmax(r)) < (unsigned)(tau >> 32)) continue;
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const u64 k = key_of(f[i], c0 + i);
-                    if (k >= tau && c0 + i >= 0 && c0 + i < a.M) {
-                        const int p = atomicAdd(&s_top.ncand, 1);
-                        if (p < kCand) s_top.cand[p] = k;
+                    for (int e = 0; e < VE; ++e) {
+                        const u64 k = key_of(element<T>(r, e), c0 + e);
+                        if (k >= tau && c0 + e >= 0 && c0 + e < a.M) {
+                            const int p = atomicAdd(&s_top.ncand, 1);
+                            if (p < kCand) s_top.cand[p] = k;
+                        }
                     }
                 }
             }
             __syncthreads();
             n_local = s_top.ncand;
             if (n_local <= kCand) break;
-            // more than fit: the K-th best of any kCand of them is a higher bound, and drops at least kCand - K
-            for (int i = tid; i < kCand; i += THREADS) {
+            // more than fit: the K-th best of any kSample of them is a higher bound, which drops kSample - K at least
+            for (int i = tid; i < kSample; i += THREADS) {
                 const u64 k = s_top.cand[i];
                 int n = 0;
-                for (int j = 0; j < kCand; ++j) n += s_top.cand[j] > k;
+                for (int j = 0; j < kSample; ++j) n += s_top.cand[j] > k;
                 if (n == a.K - 1) s_top.tau = k;
             }
             __syncthreads();
@@ -606,8 +656,8 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
     if (warp == 0) {
         Sums w = C > 1 ? (lane < C ? s_rank[lane] : Sums{0.0f, 0.0f, 0.0f}) : s_warp[0];
         if (C > 1) w = warp_join<ENT>(w, c);
-        const double S = (double)w.S;
-        double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + log(S);
+        const float logS = logf(w.S);
+        double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + (double)logS;
         if constexpr (LIST != kNone) {
             const Teacher t = warp_teacher<LIST == kTail, LIST == kTail>(s_list.l, a.K, a.inv_t);
             const double rest = lse;
@@ -633,17 +683,16 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
                 if (a.rest) a.rest[row] = (float)rest;
             }
         } else if (lane == 0) {
-            const double logS = log(S);
             a.lse[row] = (float)lse;
             // from the difference to ref, so that a large common offset costs nothing
             if (a.logp)
                 a.logp[row] = token < 0                ? 0.0f
                               : token >= a.M           ? NAN
                               : x_token == -INFINITY   ? (isnan(lse) ? NAN : -INFINITY)
-                                                       : (float)(((double)x_token - (double)w.ref) * a.inv_t - logS);
-            if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)(logS - kLn2 * ((double)w.E / S));
+                                                       : (float)(((double)x_token - (double)w.ref) * a.inv_t - (double)logS);
+            if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)((double)logS - kLn2 * (double)(w.E / w.S));
             s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
-            s_log = logS;
+            s_log = (double)logS;
         }
     }
     if constexpr (TOP) {
@@ -658,14 +707,16 @@ __global__ void __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 8) row_stats(con
             int above = 0;
             for (int j = 0; j < n; ++j) above += from[j] > k;
             if (above >= a.K) continue;
-            const float v = value_of((unsigned)(k >> 32));
+            const float x = value_of((unsigned)(k >> 32));
             const long long o = row * a.K + above;
-            a.top[o] = broken ? NAN : v == -INFINITY ? v : (float)(((double)v - row_ref) * a.inv_t - row_log);
+            a.top[o] = broken ? NAN : x == -INFINITY ? x : (float)(((double)x - row_ref) * a.inv_t - row_log);
             const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
             if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
             else static_cast<int *>(a.at)[o] = (int)col;
         }
     }
+    __syncthreads();     // before the next row's values come into the shared memory that this one's are read from
+  }
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------
@@ -681,7 +732,7 @@ struct GradArgs {
 // within a CTA: in place needs parts = 1 there).
 template <typename T, int THREADS, int LIST>
 __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int parts) {
-    constexpr int VE = Elem<T>::VE, U = 4;
+    constexpr int VE = Elem<T>::VE, U = 2;
     __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kRenorm> s_list;
     __shared__ Teacher s_teacher;
     const RowArgs &a = g.r;
@@ -692,7 +743,7 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
     const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
     T *dr = static_cast<T *>(g.dx) + row * g.lddx;
     const Row<T> rv(xr, a.M);
-    const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15u) == 0;
+    const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 31u) == 0;
     const float c = (float)(kLog2eD * a.inv_t);
 
     // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the token's
@@ -700,24 +751,25 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
     // low part, because its rounding would scale the whole row.
     double base = (double)g.lse[row];
     float al = 0.0f, be = 0.0f, gamma = 0.0f;
-    int tok_v = -1, tok_i = 0;                // vector and place of the token
+    long long token = -1;                     // its column, where this thread writes it
+    float x_token = 0.0f;
     double w = 0.0, W = 0.0, row_lse = base;
     bool broken = false;
     const bool dead = base == -INFINITY;      // no finite logit in the row: no gradient
     if constexpr (LIST == kNone) {
-        const long long token = a.tokens ? load_index(a.tokens, row, a.wide) : -1;
+        if (a.tokens) token = load_index(a.tokens, row, a.wide);
         const double dl = g.dlogp && token >= 0 ? (double)g.dlogp[row] : 0.0;
         const double de = g.dentropy ? (double)g.dentropy[row] : 0.0;
         if (!dead) {
             al = (float)((-dl - (g.dentropy ? de * (double)g.entropy[row] : 0.0)) * a.inv_t);
             be = (float)(-de * kLn2 * a.inv_t);
             gamma = (float)(dl * a.inv_t);
-            if (token >= 0 && token < a.M) {
-                tok_v = (int)((token + rv.mis) / VE);
-                tok_i = (int)((token + rv.mis) % VE);
-            }
         }
         if (token >= a.M) al = NAN;
+        if (token >= 0 && token < a.M && !dead && (int)((token + rv.mis) / VE) % total == me)
+            x_token = Elem<T>::to_float(xr[token]);      // before it may be written over
+        else
+            token = -1;
     } else {
         load_list(s_list.l, a, row, xr);
         if (tid < 32) {
@@ -744,44 +796,46 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
     base /= a.inv_t;
     const float hi = (float)base, lo = (float)((base - (double)hi) * (double)c);
 
-    auto put = [&](const uint4 &r, int v, bool whole) {
-        float f[VE];
-        Elem<T>::unpack(r, f);
+    auto slope = [&](float x) {
+        const float t = fmaf(x - hi, c, -lo);
+        const float e = pb::ex2_approx(t);
+        return LIST == kNone ? e * fmaf(be, fmaxf(t, -1e30f), al) : e * al;
+    };
+    auto put = [&](const Vec &r, int at, bool whole) {
+        Vec o;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            const float t = fmaf(f[i] - hi, c, -lo);
-            const float e = pb::ex2_approx(t);
-            f[i] = LIST == kNone ? e * fmaf(be, fmaxf(t, -1e30f), al) : e * al;
+        for (int i = 0; i < VE / 2; ++i) {
+            float x0, x1;
+            Elem<T>::pair(r, i, x0, x1);
+            Elem<T>::set_pair(o, i, slope(x0), slope(x1));
         }
-        if constexpr (LIST == kNone) {
-            if (v == tok_v) {
-#pragma unroll
-                for (int i = 0; i < VE; ++i)
-                    if (i == tok_i) f[i] += gamma;
-            }
-        }
-        const int c0 = rv.first(v);
+        const int c0 = rv.first(at);
         if (whole && same) {
-            __stcs(reinterpret_cast<uint4 *>(dr + c0), Elem<T>::pack(f));
+            st_stream(dr + c0, o);
         } else {
+            const T *e = reinterpret_cast<const T *>(o.w);
 #pragma unroll
             for (int i = 0; i < VE; ++i)
-                if (c0 + i >= 0 && c0 + i < a.M) dr[c0 + i] = Elem<T>::from_float(f[i]);
+                if (c0 + i >= 0 && c0 + i < a.M) dr[c0 + i] = e[i];
         }
     };
 
     if (rv.v0 && me == 0) put(rv.edge(0), 0, false);
-    for (int v = me < rv.v0 ? me + total : me; v < rv.v1; v += U * total) {
-        uint4 r[U];
+    {
+        int v = me < rv.v0 ? me + total : me;
+        for (; v + (U - 1) * total < rv.v1; v += U * total) {
+            Vec r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v + u * total < rv.v1) r[u] = __ldcs(rv.at(v + u * total));
+            for (int u = 0; u < U; ++u) r[u] = ld_stream(rv.at(v + u * total));
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v + u * total < rv.v1) put(r[u], v + u * total, true);
+            for (int u = 0; u < U; ++u) put(r[u], v + u * total, true);
+        }
+        for (; v < rv.v1; v += total) put(ld_stream(rv.at(v)), v, true);
     }
-    if (rv.nvec > rv.v1 && (rv.nvec > 1 || !rv.v0) && me == rv.v1 % total) put(rv.edge(rv.v1), rv.v1, false);
-    if constexpr (LIST != kNone) {
+    if (rv.tail() && me == rv.v1 % total) put(rv.edge(rv.v1), rv.v1, false);
+    if constexpr (LIST == kNone) {
+        if (token >= 0) dr[token] = Elem<T>::from_float(slope(x_token) + gamma);     // over this thread's own value
+    } else {
         // the listed columns of this part's vectors, over what the pass wrote there (each column is listed once)
         __syncthreads();
         const float norm = s_teacher.norm;
@@ -813,11 +867,17 @@ int32_t check_rows(const char *what, const void *x, int32_t dtype, int64_t ldx, 
     return PB_OK;
 }
 
-template <typename K>
-int32_t launch_clustered(K kernel, unsigned grid, unsigned threads, int C, cudaStream_t stream, const RowArgs &a) {
+template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
+int32_t launch_row_stats(const char *what, const RowArgs &a, int C, const pb::DeviceInfo &dev, cudaStream_t stream) {
+    auto kernel = row_stats<T, THREADS, ENT, TOP, LIST>;
+    int per_sm = 1;
+    PB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, THREADS, 0));
+    // a row for each cluster, or as many CTAs as are resident, which take rows in turn
+    const long long grid = C > 1 ? a.N * C : std::min<long long>(a.N, (long long)std::max(per_sm, 1) * dev.sm_count);
+    PB_REQUIRE(grid <= INT_MAX, "%s: %lld rows are too many", what, a.N);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -834,13 +894,12 @@ int32_t launch_stats(const char *what, const RowArgs &a, cudaStream_t stream) {
     const int32_t rc = pb::device_info(&dev);
     if (rc) return rc;
     const long long bytes = (long long)a.M * sizeof(T);
-    const bool big = bytes >= 512 * 16 * 2;
-    const int threads = big ? 512 : 128;
+    const bool big = bytes >= 256 * 32;
+    const int threads = big ? 256 : 128;
     int C = 1;
-    while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 16 * 2) C *= 2;
-    PB_REQUIRE(a.N * C <= INT_MAX, "%s: %lld rows are too many", what, a.N);
-    if (big) return launch_clustered(row_stats<T, 512, ENT, TOP, LIST>, (unsigned)(a.N * C), 512, C, stream, a);
-    return launch_clustered(row_stats<T, 128, ENT, TOP, LIST>, (unsigned)(a.N * C), 128, C, stream, a);
+    while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 32) C *= 2;
+    return big ? launch_row_stats<T, 256, ENT, TOP, LIST>(what, a, C, dev, stream)
+               : launch_row_stats<T, 128, ENT, TOP, LIST>(what, a, C, dev, stream);
 }
 
 template <typename T>
