@@ -19,6 +19,9 @@
 
 #include <algorithm>
 #include <climits>
+#ifdef SCAN_ENV
+#include <cstdlib>
+#endif
 
 #include "../../include/parpy_b200.h"
 #include "common.cuh"
@@ -94,14 +97,64 @@ __device__ __forceinline__ void store_word(T *p, int lane, int n, unsigned w) {
     }
 }
 
+// ---- the CH channels of a lane as one value: a register, or a pair with one instruction for both -----------------
+template <int CH>
+struct Lanes;
+template <>
+struct Lanes<1> {
+    float v;
+    __device__ static Lanes of(float a) { return {a}; }
+    __device__ static Lanes of(const float (&a)[1]) { return {a[0]}; }
+    __device__ void get(float (&a)[1]) const { a[0] = v; }
+};
+template <>
+struct Lanes<2> {
+    unsigned long long v;
+    __device__ static Lanes of(float a, float b) {
+        Lanes r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+        return r;
+    }
+    __device__ static Lanes of(float a) { return of(a, a); }
+    __device__ static Lanes of(const float (&a)[2]) { return of(a[0], a[1]); }
+    __device__ void get(float (&a)[2]) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a[0]), "=f"(a[1]) : "l"(v)); }
+};
+__device__ __forceinline__ Lanes<1> operator+(Lanes<1> a, Lanes<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Lanes<1> operator*(Lanes<1> a, Lanes<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Lanes<1> fma(Lanes<1> a, Lanes<1> b, Lanes<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Lanes<2> operator+(Lanes<2> a, Lanes<2> b) {
+    Lanes<2> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Lanes<2> operator*(Lanes<2> a, Lanes<2> b) {
+    Lanes<2> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
+    Lanes<2> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 // f = sigmoid(g) and 1 - f, each to its own relative precision: with e = exp(-g), f = 1 / (1 + e) and 1 - f = e f.
 // The exponent is capped so that e f stays 1 for g far below zero; a NaN passes.
-__device__ __forceinline__ void gate(float g, float &f, float &keep) {
-    float t = -1.4426950408889634f * g;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(t), "f"(126.0f));
-    const float e = pb::ex2_approx(t);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(1.0f + e));
-    keep = e * f;
+template <int CH>
+__device__ __forceinline__ void gate(const float (&g)[CH], Lanes<CH> &f, Lanes<CH> &keep) {
+    float t[CH], e[CH], d[CH], r[CH];
+    (Lanes<CH>::of(g) * Lanes<CH>::of(-1.4426950408889634f)).get(t);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(t[j]) : "f"(t[j]), "f"(126.0f));
+        e[j] = pb::ex2_approx(t[j]);
+    }
+    const Lanes<CH> el = Lanes<CH>::of(e);
+    (el + Lanes<CH>::of(1.0f)).get(d);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[j]) : "f"(d[j]));
+    f = Lanes<CH>::of(r);
+    keep = el * f;
 }
 
 __device__ __forceinline__ void st_cluster_f32x2(unsigned addr, float a, float b) {
@@ -133,26 +186,41 @@ __device__ __forceinline__ T *start_of(const Walk &w, int b, int c0) {
     return static_cast<T *>(w.p) + b * w.sb + c0;
 }
 
-// grid.x = sequences x channel blocks x C; a cluster of C CTAs works on C tiles of one sequence at a time.
+// The steps of a warp's run, a fixed number of rows apart. The warp's number is broadcast so that addresses and bounds
+// are known to be the same for all lanes.
+template <typename T, bool VEC, int S>
+__device__ __forceinline__ void load_run(unsigned (&w)[S], const T *p, long long st, int steps, int lane, int n) {
+    if (steps >= S) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) w[s] = load_word<T, VEC>(p + s * st, lane, n);
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s) w[s] = s < steps ? load_word<T, VEC>(p + s * st, lane, n) : 0u;
+    }
+}
+
+// grid.x = sequences x channel blocks x C; a cluster of C CTAs works on C tiles of one sequence at a time. A round: every
+// warp folds its run; one warp per channel plane folds the tile's runs, exchanges the tile's (A, B) within the cluster
+// and leaves the state that enters each run; every warp steps through its run. The next round's inputs are in
+// registers before the exchange begins.
 template <typename T, bool VEC, int S, int W>
 __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, const int C) {
     static_assert(S * W == kTile, "one stored state per tile");
     constexpr int CH = Word<T>::CH;
-    __shared__ float2 s_run[2][W][CH][32];
-    __shared__ float2 s_tile[2][kMaxRanks][CH][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    using L = Lanes<CH>;
+    __shared__ float2 s_run[W][CH][32];              // (A, B) of each run
+    __shared__ float s_in[W][CH][32];                // state entering each run
+    __shared__ float2 s_tile[2][kMaxRanks][CH][32];  // (A, B) of the cluster's tiles, by round parity
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
     const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
     const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
     const T *g = start_of<T>(a.g, b, c0), *x = start_of<T>(a.x, b, c0);
     T *h = start_of<T>(a.h, b, c0);
 
-    float state[CH];      // entering the cluster's tiles of this round
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        const int c = channel<T, VEC>(lane, j);
-        state[j] = a.h0 && c < n ? a.h0[(long long)b * a.D + c0 + c] : 0.0f;
-    }
+    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
+    const int mine = channel<T, VEC>(lane, warp);
+    if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
     if (C > 1) {          // every CTA runs before the first store into its shared memory
         cluster_arrive();
         cluster_wait();
@@ -160,137 +228,130 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
     const int stride = C * kTile, rounds = (len + stride - 1) / stride;
     int t0 = rank * kTile + warp * S;
     unsigned gw[S], xw[S];
-    auto fetch = [&](int t) {
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            gw[s] = xw[s] = 0;
-            if (t + s < len) {
-                gw[s] = load_word<T, VEC>(g + (t + s) * a.g.st, lane, n);
-                xw[s] = load_word<T, VEC>(x + (t + s) * a.x.st, lane, n);
-            }
-        }
-    };
-    fetch(t0);
+    load_run<T, VEC, S>(gw, g + t0 * a.g.st, a.g.st, len - t0, lane, n);
+    load_run<T, VEC, S>(xw, x + t0 * a.x.st, a.x.st, len - t0, lane, n);
     for (int round = 0; round < rounds; ++round, t0 += stride) {
         const int par = round & 1;
-        float f[S][CH], u[S][CH], A[CH], Bv[CH];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            A[j] = 1.0f;
-            Bv[j] = 0.0f;
-        }
+        L f[S], u[S], A = L::of(1.0f), B = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH];
             Word<T>::unpack(gw[s], gv);
             Word<T>::unpack(xw[s], xv);
-            const bool in = t0 + s < len;
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                float keep;
-                gate(gv[j], f[s][j], keep);
-                u[s][j] = keep * xv[j];
-                if (!in) {            // behind the end the state is held
-                    f[s][j] = 1.0f;
-                    u[s][j] = 0.0f;
-                }
-                A[j] *= f[s][j];
-                Bv[j] = fmaf(f[s][j], Bv[j], u[s][j]);
-            }
+            gate<CH>(gv, f[s], u[s]);
+            u[s] = u[s] * L::of(xv);
         }
-        if (round + 1 < rounds) fetch(t0 + stride);
+        if (t0 + S > len) {           // behind the end the state is held
 #pragma unroll
-        for (int j = 0; j < CH; ++j) s_run[par][warp][j][lane] = make_float2(A[j], Bv[j]);
+            for (int s = 0; s < S; ++s)
+                if (t0 + s >= len) {
+                    f[s] = L::of(1.0f);
+                    u[s] = L::of(0.0f);
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            A = A * f[s];
+            B = fma(f[s], B, u[s]);
+        }
+        {
+            float av[CH], bv[CH];
+            A.get(av);
+            B.get(bv);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) s_run[warp][j][lane] = make_float2(av[j], bv[j]);
+        }
+        if (round + 1 < rounds) {
+            const long long t = t0 + stride;
+            load_run<T, VEC, S>(gw, g + t * a.g.st, a.g.st, len - (int)t, lane, n);
+            load_run<T, VEC, S>(xw, x + t * a.x.st, a.x.st, len - (int)t, lane, n);
+        }
         __syncthreads();
-        float pa[CH], pb[CH], ta[CH], tb[CH];    // runs before this warp's, and the whole tile
+        float2 run[W];
+        if (warp < CH) {
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            ta[j] = 1.0f;
-            tb[j] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                if (w == warp) {
-                    pa[j] = ta[j];
-                    pb[j] = tb[j];
-                }
-                const float2 r = s_run[par][w][j][lane];
-                ta[j] *= r.x;
-                tb[j] = fmaf(r.x, tb[j], r.y);
-            }
+            for (int w = 0; w < W; ++w) run[w] = s_run[w][warp][lane];
         }
-        float in[CH];
         if (C > 1) {
-            if (warp == 0) {
-                for (int r = 0; r < C; ++r)
+            if (warp < CH) {
+                float ta = 1.0f, tb = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        st_cluster_f32x2(map_to_rank(smem_u32(&s_tile[par][rank][j][lane]), r), ta[j], tb[j]);
+                for (int w = 0; w < W; ++w) {
+                    ta *= run[w].x;
+                    tb = fmaf(run[w].x, tb, run[w].y);
+                }
+                const unsigned at = smem_u32(&s_tile[par][rank][warp][lane]);
+                for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), ta, tb);
             }
             cluster_arrive();
             cluster_wait();
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
+        }
+        if (warp < CH) {
+            float in = state;
+            if (C > 1) {
                 for (int r = 0; r < C; ++r) {
-                    if (r == rank) in[j] = state[j];
-                    const float2 v = s_tile[par][r][j][lane];
-                    state[j] = fmaf(v.x, state[j], v.y);
+                    if (r == rank) in = state;
+                    const float2 v = s_tile[par][r][warp][lane];
+                    state = fmaf(v.x, state, v.y);
                 }
+            }
+            const int tile = round * C + rank;
+            if (a.carry && mine < n && tile * kTile < len)
+                a.carry[((long long)b * ((a.T + kTile - 1) / kTile) + tile) * a.D + c0 + mine] = in;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                s_in[w][warp][lane] = in;
+                in = fmaf(run[w].x, in, run[w].y);
+            }
+            if (C == 1) state = in;
+        }
+        __syncthreads();
+        float v[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] = s_in[warp][j][lane];
+        L hs = L::of(v);
+        T *out = h + t0 * a.h.st;
+        if (t0 + S <= len) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                hs = fma(f[s], hs, u[s]);
+                hs.get(v);
+                store_word<T, VEC>(out + s * a.h.st, lane, n, Word<T>::pack(v));
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                in[j] = state[j];
-                state[j] = fmaf(ta[j], state[j], tb[j]);
+            for (int s = 0; s < S; ++s) {
+                hs = fma(f[s], hs, u[s]);
+                hs.get(v);
+                if (t0 + s < a.T) store_word<T, VEC>(out + s * a.h.st, lane, n, t0 + s < len ? Word<T>::pack(v) : 0u);
             }
-        }
-        const int tile = round * C + rank;
-        if (a.carry && warp == 0 && tile * kTile < len) {
-            const long long at = ((long long)b * ((a.T + kTile - 1) / kTile) + tile) * a.D + c0;
-#pragma unroll
-            for (int j = 0; j < CH; ++j)
-                if (channel<T, VEC>(lane, j) < n) a.carry[at + channel<T, VEC>(lane, j)] = in[j];
-        }
-        float v[CH];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) v[j] = fmaf(pa[j], in[j], pb[j]);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool alive = t0 + s < len;
-#pragma unroll
-            for (int j = 0; j < CH; ++j) v[j] = fmaf(f[s][j], v[j], u[s][j]);
-            if (t0 + s < a.T) store_word<T, VEC>(h + (t0 + s) * a.h.st, lane, n, alive ? Word<T>::pack(v) : 0u);
         }
     }
     for (; t0 < a.T; t0 += stride)     // behind the end
         for (int s = 0; s < S && t0 + s < a.T; ++s) store_word<T, VEC>(h + (t0 + s) * a.h.st, lane, n, 0u);
-    if (a.last && rank == 0 && warp == 0) {
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (channel<T, VEC>(lane, j) < n) a.last[(long long)b * a.D + c0 + channel<T, VEC>(lane, j)] = state[j];
-    }
+    if (a.last && rank == 0 && warp < CH && mine < n) a.last[(long long)b * a.D + c0 + mine] = state;
 }
 
 template <typename T, bool VEC, int S, int W>
 __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const int C) {
     static_assert(S * W == kTile, "one stored state per tile");
     constexpr int CH = Word<T>::CH;
-    __shared__ float2 s_run[2][W][CH][32];      // (A, B) of the states
-    __shared__ float s_back[2][W][CH][32];      // B of the gradients; their A is the same product
+    using L = Lanes<CH>;
+    __shared__ float2 s_run[W][CH][32];              // (A, B) of each run's states
+    __shared__ float s_back[W][CH][32];              // B of each run's gradients; their A is the same product
+    __shared__ float s_in[W][CH][32], s_out[W][CH][32];     // state entering each run; c entering it from behind
     __shared__ float2 s_tile[2][kMaxRanks][CH][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
     const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
     const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
-    const T *g = start_of<T>(a.g, b, c0), *x = start_of<T>(a.x, b, c0), *dh = a.dh.p ? start_of<T>(a.dh, b, c0) : nullptr;
+    const T *g = start_of<T>(a.g, b, c0), *x = start_of<T>(a.x, b, c0), *dh = start_of<T>(a.dh, b, c0);
     T *dg = start_of<T>(a.dg, b, c0), *dx = start_of<T>(a.dx, b, c0);
-    const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0;
+    const int plane = warp < CH ? warp : warp - CH, mine = channel<T, VEC>(lane, plane);
+    const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
 
-    float back[CH];       // c entering the cluster's tiles of this round from behind
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        const int c = channel<T, VEC>(lane, j);
-        back[j] = a.dlast && c < n ? a.dlast[(long long)b * a.D + c0 + c] : 0.0f;
-    }
+    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
+    if (warp < CH && a.dlast && mine < n) back = a.dlast[(long long)b * a.D + c0 + mine];
     if (C > 1) {
         cluster_arrive();
         cluster_wait();
@@ -303,143 +364,137 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
         }
     int t0 = (rounds - 1) * stride + rank * kTile + warp * S;
     unsigned gw[S], xw[S], dw[S];
-    float cv[CH];         // the stored state of the tile
-    auto fetch = [&](int t, int tile) {
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            gw[s] = xw[s] = dw[s] = 0;
-            if (t + s < len) {
-                gw[s] = load_word<T, VEC>(g + (t + s) * a.g.st, lane, n);
-                xw[s] = load_word<T, VEC>(x + (t + s) * a.x.st, lane, n);
-                if (dh) dw[s] = load_word<T, VEC>(dh + (t + s) * a.dh.st, lane, n);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            const int c = channel<T, VEC>(lane, j);
-            cv[j] = c < n && tile * kTile < len ? carry[(long long)tile * a.D + c] : 0.0f;
-        }
+    float stored = 0.0f;  // of the second set of planes' warps: the state at the start of the tile
+    auto fetch = [&](long long t, int tile) {
+        load_run<T, VEC, S>(gw, g + t * a.g.st, a.g.st, len - (int)t, lane, n);
+        load_run<T, VEC, S>(xw, x + t * a.x.st, a.x.st, len - (int)t, lane, n);
+        load_run<T, VEC, S>(dw, dh + t * a.dh.st, a.dh.st, a.dh.p ? len - (int)t : 0, lane, n);
+        if (warp >= CH && warp < 2 * CH) stored = mine < n && tile * kTile < len ? carry[(long long)tile * a.D] : 0.0f;
     };
     if (rounds > 0) fetch(t0, (rounds - 1) * C + rank);
     for (int round = rounds - 1; round >= 0; --round, t0 -= stride) {
         const int par = round & 1;
-        float f[S][CH], keep[S][CH], xv[S][CH], d[S][CH], hp[CH], A[CH], Bv[CH], Rv[CH];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            A[j] = 1.0f;
-            Bv[j] = Rv[j] = 0.0f;
-            hp[j] = cv[j];
-        }
+        L f[S], keep[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
+        unsigned xn[S], dn[S];
+        const float entering = stored;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH];
             Word<T>::unpack(gw[s], gv);
-            Word<T>::unpack(xw[s], xv[s]);
-            Word<T>::unpack(dw[s], d[s]);
-            const bool in = t0 + s < len;
+            gate<CH>(gv, f[s], keep[s]);
+            xn[s] = xw[s];
+            dn[s] = dw[s];
+        }
+        if (t0 + S > len) {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (t0 + s >= len) {
+                    f[s] = L::of(1.0f);
+                    keep[s] = L::of(0.0f);
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float xv[CH];
+            Word<T>::unpack(xn[s], xv);
+            A = A * f[s];
+            B = fma(f[s], B, keep[s] * L::of(xv));
+        }
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+            float dv[CH];
+            Word<T>::unpack(dn[s], dv);
+            R = f[s] * (L::of(dv) + R);
+        }
+        {
+            float av[CH], bv[CH], rv[CH];
+            A.get(av);
+            B.get(bv);
+            R.get(rv);
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-                gate(gv[j], f[s][j], keep[s][j]);
-                if (!in) {
-                    f[s][j] = 1.0f;
-                    keep[s][j] = 0.0f;
-                }
-                A[j] *= f[s][j];
-                Bv[j] = fmaf(f[s][j], Bv[j], keep[s][j] * xv[s][j]);
+                s_run[warp][j][lane] = make_float2(av[j], bv[j]);
+                s_back[warp][j][lane] = rv[j];
             }
         }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s)
-#pragma unroll
-            for (int j = 0; j < CH; ++j) Rv[j] = f[s][j] * (d[s][j] + Rv[j]);
         if (round > 0) fetch(t0 - stride, (round - 1) * C + rank);
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            s_run[par][warp][j][lane] = make_float2(A[j], Bv[j]);
-            s_back[par][warp][j][lane] = Rv[j];
-        }
         __syncthreads();
-        float qa[CH], qb[CH];      // the runs behind this warp's, then the whole tile
-        float ra[CH], rb[CH];
+        if (warp >= CH && warp < 2 * CH) {
+            float in = entering;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-                if (w < warp) {
-                    const float2 r = s_run[par][w][j][lane];
-                    hp[j] = fmaf(r.x, hp[j], r.y);
-                }
-            qa[j] = 1.0f;
-            qb[j] = 0.0f;
-#pragma unroll
-            for (int w = W - 1; w >= 0; --w) {
-                if (w == warp) {
-                    ra[j] = qa[j];
-                    rb[j] = qb[j];
-                }
-                const float aw = s_run[par][w][j][lane].x;
-                qa[j] *= aw;
-                qb[j] = fmaf(aw, qb[j], s_back[par][w][j][lane]);
+            for (int w = 0; w < W; ++w) {
+                const float2 r = s_run[w][plane][lane];
+                s_in[w][plane][lane] = in;
+                in = fmaf(r.x, in, r.y);
             }
         }
-        float in[CH];
         if (C > 1) {
-            if (warp == 0) {
-                for (int r = 0; r < C; ++r)
+            if (warp < CH) {
+                float qa = 1.0f, qb = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        st_cluster_f32x2(map_to_rank(smem_u32(&s_tile[par][rank][j][lane]), r), qa[j], qb[j]);
+                for (int w = W - 1; w >= 0; --w) {
+                    const float aw = s_run[w][plane][lane].x;
+                    qa *= aw;
+                    qb = fmaf(aw, qb, s_back[w][plane][lane]);
+                }
+                const unsigned at = smem_u32(&s_tile[par][rank][plane][lane]);
+                for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), qa, qb);
             }
             cluster_arrive();
             cluster_wait();
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
+        }
+        if (warp < CH) {
+            float out = back;
+            if (C > 1) {
                 for (int r = C - 1; r >= 0; --r) {
-                    if (r == rank) in[j] = back[j];
-                    const float2 v = s_tile[par][r][j][lane];
-                    back[j] = fmaf(v.x, back[j], v.y);
+                    if (r == rank) out = back;
+                    const float2 v = s_tile[par][r][plane][lane];
+                    back = fmaf(v.x, back, v.y);
                 }
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                in[j] = back[j];
-                back[j] = fmaf(qa[j], back[j], qb[j]);
+            for (int w = W - 1; w >= 0; --w) {
+                s_out[w][plane][lane] = out;
+                out = fmaf(s_run[w][plane][lane].x, out, s_back[w][plane][lane]);
             }
+            if (C == 1) back = out;
         }
+        __syncthreads();
         // the states before each step, then backwards through the run
-        float before[S][CH], c[CH];
+        float v[CH];
+        L before[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+        for (int j = 0; j < CH; ++j) v[j] = s_in[warp][j][lane];
+        L hs = L::of(v);
 #pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                before[s][j] = hp[j];
-                hp[j] = fmaf(f[s][j], hp[j], keep[s][j] * xv[s][j]);
-            }
+        for (int s = 0; s < S; ++s) {
+            float xv[CH];
+            Word<T>::unpack(xn[s], xv);
+            before[s] = hs;
+            hs = fma(f[s], hs, keep[s] * L::of(xv));
+        }
 #pragma unroll
-        for (int j = 0; j < CH; ++j) c[j] = fmaf(ra[j], in[j], rb[j]);
+        for (int j = 0; j < CH; ++j) v[j] = s_out[warp][j][lane];
+        L c = L::of(v);
+        T *const ox = dx + t0 * a.dx.st, *const og = dg + t0 * a.dg.st;
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
-            float gx[CH], gg[CH];
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const float r = d[s][j] + c[j];
-                gx[j] = keep[s][j] * r;
-                gg[j] = gx[j] * f[s][j] * (before[s][j] - xv[s][j]);
-                c[j] = f[s][j] * r;
-            }
+            float xv[CH], dv[CH], gx[CH], gg[CH];
+            Word<T>::unpack(xn[s], xv);
+            Word<T>::unpack(dn[s], dv);
+            const L r = L::of(dv) + c, kr = keep[s] * r;
+            const L gl = kr * f[s] * fma(L::of(xv), L::of(-1.0f), before[s]);
+            c = f[s] * r;
+            kr.get(gx);
+            gl.get(gg);
             if (t0 + s < a.T) {
                 const bool alive = t0 + s < len;
-                store_word<T, VEC>(dx + (t0 + s) * a.dx.st, lane, n, alive ? Word<T>::pack(gx) : 0u);
-                store_word<T, VEC>(dg + (t0 + s) * a.dg.st, lane, n, alive ? Word<T>::pack(gg) : 0u);
+                store_word<T, VEC>(ox + s * a.dx.st, lane, n, alive ? Word<T>::pack(gx) : 0u);
+                store_word<T, VEC>(og + s * a.dg.st, lane, n, alive ? Word<T>::pack(gg) : 0u);
             }
         }
     }
-    if (a.dh0 && rank == 0 && warp == 0) {
-#pragma unroll
-        for (int j = 0; j < CH; ++j)
-            if (channel<T, VEC>(lane, j) < n) a.dh0[(long long)b * a.D + c0 + channel<T, VEC>(lane, j)] = back[j];
-    }
+    if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
 }
 
 // ---- one token for every row: 8 channels per thread where the rows allow 16-byte access, else one ------------
@@ -473,9 +528,10 @@ __global__ void __launch_bounds__(256) scan_step(const T *g, const T *x, const f
     }
 #pragma unroll
     for (int k = 0; k < VN; ++k) {
-        float f, keep;
-        gate((float)gv[k], f, keep);
-        lv[k] = fmaf(f, sv[k], keep * (float)xv[k]);
+        const float gk[1] = {(float)gv[k]};
+        Lanes<1> f, keep;
+        gate<1>(gk, f, keep);
+        lv[k] = fmaf(f.v, sv[k], keep.v * (float)xv[k]);
         hv[k] = (T)lv[k];
     }
     if constexpr (VN == 1) {
@@ -543,6 +599,9 @@ int32_t launch_scan(K kernel, const char *what, ScanArgs &a, int channels, int t
 
 int cluster_of(const ScanArgs &a, int channels, int sms) {
     const long long blocks = (long long)a.B * ((a.D + channels - 1) / channels);
+#ifdef SCAN_ENV
+    if (getenv("SCAN_C")) return atoi(getenv("SCAN_C"));
+#endif
     int C = 1;
     while (C < kMaxRanks && blocks * C < 2LL * sms && (long long)C * kTile < a.T) C *= 2;
     return C;
