@@ -31,6 +31,21 @@ namespace {
 
 constexpr int kTile = PARPY_B200_SCAN_TILE;   // steps per tile, and per stored state
 constexpr int kMaxRanks = 8;
+#ifndef SCAN_FB
+#define SCAN_FB 2
+#endif
+#ifndef SCAN_FN
+#define SCAN_FN 3
+#endif
+#ifndef SCAN_BB
+#define SCAN_BB 1
+#endif
+#ifndef SCAN_BN
+#define SCAN_BN 3
+#endif
+#ifndef SCAN_BS
+#define SCAN_BS 8
+#endif
 
 // ---- four bytes of a row: the channels of one lane ------------------------------------------------------
 template <typename T>
@@ -98,6 +113,7 @@ __device__ __forceinline__ void store_word(T *p, int lane, int n, unsigned w) {
 }
 
 // ---- the CH channels of a lane as one value: a register, or a pair with one instruction for both -----------------
+// Nothing is contracted behind the source's back, so that all layouts give the same bits.
 template <int CH>
 struct Lanes;
 template <>
@@ -119,8 +135,8 @@ struct Lanes<2> {
     __device__ static Lanes of(const float (&a)[2]) { return of(a[0], a[1]); }
     __device__ void get(float (&a)[2]) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a[0]), "=f"(a[1]) : "l"(v)); }
 };
-__device__ __forceinline__ Lanes<1> operator+(Lanes<1> a, Lanes<1> b) { return {a.v + b.v}; }
-__device__ __forceinline__ Lanes<1> operator*(Lanes<1> a, Lanes<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Lanes<1> operator+(Lanes<1> a, Lanes<1> b) { return {__fadd_rn(a.v, b.v)}; }
+__device__ __forceinline__ Lanes<1> operator*(Lanes<1> a, Lanes<1> b) { return {__fmul_rn(a.v, b.v)}; }
 __device__ __forceinline__ Lanes<1> fma(Lanes<1> a, Lanes<1> b, Lanes<1> c) { return {fmaf(a.v, b.v, c.v)}; }
 __device__ __forceinline__ Lanes<2> operator+(Lanes<2> a, Lanes<2> b) {
     Lanes<2> r;
@@ -401,11 +417,12 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
             B = fma(f[s], B, keep[s] * L::of(xv));
         }
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
+        for (int s = S - 1; s >= 0; --s) {       // r_s = dh_s + f_{s+1} r_{s+1}
             float dv[CH];
             Word<T>::unpack(dn[s], dv);
-            R = f[s] * (L::of(dv) + R);
+            R = s == S - 1 ? L::of(dv) : fma(f[s + 1 < S ? s + 1 : s], R, L::of(dv));
         }
+        R = f[0] * R;
         {
             float av[CH], bv[CH], rv[CH];
             A.get(av);
@@ -475,16 +492,15 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
         }
 #pragma unroll
         for (int j = 0; j < CH; ++j) v[j] = s_out[warp][j][lane];
-        L c = L::of(v);
+        L r = L::of(v);
         T *const ox = dx + t0 * a.dx.st, *const og = dg + t0 * a.dg.st;
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
             float xv[CH], dv[CH], gx[CH], gg[CH];
             Word<T>::unpack(xn[s], xv);
             Word<T>::unpack(dn[s], dv);
-            const L r = L::of(dv) + c, kr = keep[s] * r;
-            const L gl = kr * f[s] * fma(L::of(xv), L::of(-1.0f), before[s]);
-            c = f[s] * r;
+            r = s == S - 1 ? L::of(dv) + r : fma(f[s + 1 < S ? s + 1 : s], r, L::of(dv));
+            const L kr = keep[s] * r, gl = kr * (f[s] * fma(L::of(xv), L::of(-1.0f), before[s]));
             kr.get(gx);
             gl.get(gg);
             if (t0 + s < a.T) {
@@ -494,6 +510,373 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
             }
         }
     }
+    if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
+}
+
+// ---- the same two kernels where rows allow 16-byte access ----------------------------------------------------------
+// A warp's run of S steps x 128 bytes of channels lies in S rows of shared memory that only this warp uses: fetched
+// with 16-byte asynchronous copies kStages - 1 rounds ahead, read with 4-byte loads at constant offsets, overwritten in place
+// by the results, and written back 16 bytes a lane. (Loading and storing 4 bytes a lane and step straight from global
+// memory spends two thirds of the instructions on addresses.)
+__device__ __forceinline__ void copy16(unsigned to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One array's rows of a run: row i of the run at step t + i, 128 bytes; a lane moves 16 bytes of every fourth row.
+template <typename T, int S>
+struct Rows {
+    T *p;               // this lane's place in the first row
+    long long st;
+    bool in;            // the lane's channels exist
+    int sub;            // its row within four
+    __device__ Rows(const Walk &w, int b, int c0, int n, int lane) {
+        constexpr int E = 16 / sizeof(T);
+        p = start_of<T>(w, b, c0) + (lane & 7) * E;
+        st = w.st;
+        in = w.p && (lane & 7) * E < n;
+        sub = lane >> 3;
+    }
+    __device__ void fetch(unsigned to, int t, int end, int lane) const {
+        const T *q = p + (t + sub) * st;
+        const int left = in ? end - t - sub : 0;
+#pragma unroll
+        for (int i = 0; i < S / 4; ++i)
+            if (4 * i < left) copy16(to + i * 512 + lane * 16, q + 4 * i * st);
+    }
+    __device__ void store(const uint4 *from, int t, int len, int end, int lane) const {
+        T *q = p + (t + sub) * st;
+        const int left = in ? end - t - sub : 0;
+#pragma unroll
+        for (int i = 0; i < S / 4; ++i)
+            if (4 * i < left) {
+                const uint4 v = from[i * 32 + lane];
+                __stcs(reinterpret_cast<uint4 *>(q + 4 * i * st), t + sub + 4 * i < len ? v : make_uint4(0, 0, 0, 0));
+            }
+    }
+};
+
+template <typename T, int S, int W, int NST>
+__global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const ScanArgs a, const int C) {
+    static_assert(S * W == kTile, "one stored state per tile");
+    constexpr int CH = Word<T>::CH, kRun = S * 128;       // bytes of one array's run
+    using L = Lanes<CH>;
+    extern __shared__ __align__(128) unsigned char s_rows[];
+    __shared__ float2 s_run[W][CH][32];              // (A, B) of each run
+    __shared__ float s_in[W][CH][32];                // state entering each run
+    __shared__ float2 s_tile[2][kMaxRanks][CH][32];  // (A, B) of the cluster's tiles, by round parity
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+    const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
+    const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
+    const Rows<T, S> g(a.g, b, c0, n, lane), x(a.x, b, c0, n, lane), h(a.h, b, c0, n, lane);
+    unsigned char *const mine_rows = s_rows + warp * (NST * 2 * kRun);
+    const unsigned rows = smem_u32(mine_rows);
+
+    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
+    const int mine = lane * CH + warp;
+    if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
+    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
+    int t0 = rank * kTile + warp * S, fill = 0;
+    auto fetch = [&](int t) {
+        if (t < len) {
+            g.fetch(rows + fill, t, len, lane);
+            x.fetch(rows + fill + kRun, t, len, lane);
+        }
+        copy_commit();
+        fill = fill == (NST - 1) * 2 * kRun ? 0 : fill + 2 * kRun;
+    };
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i) fetch(t0 + i * stride);
+    if (C > 1) {          // every CTA runs before the first store into its shared memory
+        cluster_arrive();
+        cluster_wait();
+    }
+    int slot = 0;
+    for (int round = 0; round < rounds; ++round, t0 += stride) {
+        const int par = round & 1;
+        fetch(t0 + (NST - 1) * stride);      // into the rows that the round before has written back
+        copy_wait<NST - 1>();
+        __syncwarp();
+        unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4;
+        slot = slot == (NST - 1) * 2 * kRun ? 0 : slot + 2 * kRun;
+        L f[S], u[S], A = L::of(1.0f), B = L::of(0.0f);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float gv[CH], xv[CH];
+            Word<T>::unpack(gr[s * 32], gv);
+            Word<T>::unpack(xr[s * 32], xv);
+            gate<CH>(gv, f[s], u[s]);
+            u[s] = u[s] * L::of(xv);
+        }
+        if (t0 + S > len) {                  // behind the end the state is held
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (t0 + s >= len) {
+                    f[s] = L::of(1.0f);
+                    u[s] = L::of(0.0f);
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            A = A * f[s];
+            B = fma(f[s], B, u[s]);
+        }
+        {
+            float av[CH], bv[CH];
+            A.get(av);
+            B.get(bv);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) s_run[warp][j][lane] = make_float2(av[j], bv[j]);
+        }
+        __syncthreads();
+        float2 run[W];
+        if (warp < CH) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) run[w] = s_run[w][warp][lane];
+        }
+        if (C > 1) {
+            if (warp < CH) {
+                float ta = 1.0f, tb = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    ta *= run[w].x;
+                    tb = fmaf(run[w].x, tb, run[w].y);
+                }
+                const unsigned at = smem_u32(&s_tile[par][rank][warp][lane]);
+                for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), ta, tb);
+            }
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (warp < CH) {
+            float in = state;
+            if (C > 1) {
+                for (int r = 0; r < C; ++r) {
+                    if (r == rank) in = state;
+                    const float2 v = s_tile[par][r][warp][lane];
+                    state = fmaf(v.x, state, v.y);
+                }
+            }
+            const int tile = round * C + rank;
+            if (a.carry && mine < n && tile * kTile < len)
+                a.carry[((long long)b * ((a.T + kTile - 1) / kTile) + tile) * a.D + c0 + mine] = in;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                s_in[w][warp][lane] = in;
+                in = fmaf(run[w].x, in, run[w].y);
+            }
+            if (C == 1) state = in;
+        }
+        __syncthreads();
+        float v[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] = s_in[warp][j][lane];
+        L hs = L::of(v);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            hs = fma(f[s], hs, u[s]);
+            hs.get(v);
+            xr[s * 32] = Word<T>::pack(v);
+        }
+        __syncwarp();
+        h.store(reinterpret_cast<const uint4 *>(xr - lane), t0, len, a.T, lane);
+        __syncwarp();
+    }
+    copy_wait<0>();
+    for (; t0 < a.T; t0 += stride) h.store(reinterpret_cast<const uint4 *>(mine_rows), t0, 0, a.T, lane);   // zeros
+    if (a.last && rank == 0 && warp < CH && mine < n) a.last[(long long)b * a.D + c0 + mine] = state;
+}
+
+template <typename T, int S, int W, int NST>
+__global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const ScanArgs a, const int C) {
+    static_assert(S * W == kTile, "one stored state per tile");
+    constexpr int CH = Word<T>::CH, kRun = S * 128;
+    using L = Lanes<CH>;
+    extern __shared__ __align__(128) unsigned char s_rows[];
+    __shared__ float2 s_run[W][CH][32];              // (A, B) of each run's states
+    __shared__ float s_back[W][CH][32];              // B of each run's gradients; their A is the same product
+    __shared__ float s_in[W][CH][32], s_out[W][CH][32];     // state entering each run; c entering it from behind
+    __shared__ float2 s_tile[2][kMaxRanks][CH][32];
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+    const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
+    const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
+    const Rows<T, S> g(a.g, b, c0, n, lane), x(a.x, b, c0, n, lane), dh(a.dh, b, c0, n, lane);
+    const Rows<T, S> dg(a.dg, b, c0, n, lane), dx(a.dx, b, c0, n, lane);
+    unsigned char *const mine_rows = s_rows + warp * (NST * 3 * kRun);
+    const unsigned rows = smem_u32(mine_rows);
+    const int plane = warp < CH ? warp : warp - CH, mine = lane * CH + plane;
+    const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
+
+    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
+    if (warp < CH && a.dlast && mine < n) back = a.dlast[(long long)b * a.D + c0 + mine];
+    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
+    for (int t = rounds * stride + rank * kTile + warp * S; t < a.T; t += stride) {      // behind the end
+        dg.store(reinterpret_cast<const uint4 *>(mine_rows), t, 0, a.T, lane);
+        dx.store(reinterpret_cast<const uint4 *>(mine_rows), t, 0, a.T, lane);
+    }
+    int t0 = (rounds - 1) * stride + rank * kTile + warp * S, fill = 0;
+    auto fetch = [&](int t) {
+        if (t >= 0 && t < len) {
+            g.fetch(rows + fill, t, len, lane);
+            x.fetch(rows + fill + kRun, t, len, lane);
+            dh.fetch(rows + fill + 2 * kRun, t, len, lane);
+        }
+        copy_commit();
+        fill = fill == (NST - 1) * 3 * kRun ? 0 : fill + 3 * kRun;
+    };
+    // a second set of planes' warps holds the state at the start of the tile, one round ahead
+    auto state_of = [&](int round) {
+        const int tile = round * C + rank;
+        return round >= 0 && warp >= CH && warp < 2 * CH && mine < n && tile * kTile < len ? carry[(long long)tile * a.D]
+                                                                                           : 0.0f;
+    };
+    float stored = state_of(rounds - 1);
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i) fetch(t0 - i * stride);
+    if (C > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    int slot = 0;
+    for (int round = rounds - 1; round >= 0; --round, t0 -= stride) {
+        const int par = round & 1;
+        fetch(t0 - (NST - 1) * stride);
+        const float entering = stored;
+        stored = state_of(round - 1);
+        copy_wait<NST - 1>();
+        __syncwarp();
+        unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4,
+                       *const dr = xr + kRun / 4;
+        slot = slot == (NST - 1) * 3 * kRun ? 0 : slot + 3 * kRun;
+        L f[S], keep[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float gv[CH];
+            Word<T>::unpack(gr[s * 32], gv);
+            gate<CH>(gv, f[s], keep[s]);
+        }
+        const bool cut = t0 + S > len;
+        if (cut) {                           // behind the end: held, and no gradient
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (t0 + s >= len) {
+                    f[s] = L::of(1.0f);
+                    keep[s] = L::of(0.0f);
+                    xr[s * 32] = 0;
+                    dr[s * 32] = 0;
+                }
+        }
+        if (!a.dh.p) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) dr[s * 32] = 0;
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float xv[CH];
+            Word<T>::unpack(xr[s * 32], xv);
+            A = A * f[s];
+            B = fma(f[s], B, keep[s] * L::of(xv));
+        }
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {       // r_s = dh_s + f_{s+1} r_{s+1}
+            float dv[CH];
+            Word<T>::unpack(dr[s * 32], dv);
+            R = s == S - 1 ? L::of(dv) : fma(f[s + 1 < S ? s + 1 : s], R, L::of(dv));
+        }
+        R = f[0] * R;
+        {
+            float av[CH], bv[CH], rv[CH];
+            A.get(av);
+            B.get(bv);
+            R.get(rv);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                s_run[warp][j][lane] = make_float2(av[j], bv[j]);
+                s_back[warp][j][lane] = rv[j];
+            }
+        }
+        __syncthreads();
+        if (warp >= CH && warp < 2 * CH) {
+            float in = entering;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 r = s_run[w][plane][lane];
+                s_in[w][plane][lane] = in;
+                in = fmaf(r.x, in, r.y);
+            }
+        }
+        if (C > 1) {
+            if (warp < CH) {
+                float qa = 1.0f, qb = 0.0f;
+#pragma unroll
+                for (int w = W - 1; w >= 0; --w) {
+                    const float aw = s_run[w][plane][lane].x;
+                    qa *= aw;
+                    qb = fmaf(aw, qb, s_back[w][plane][lane]);
+                }
+                const unsigned at = smem_u32(&s_tile[par][rank][plane][lane]);
+                for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), qa, qb);
+            }
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (warp < CH) {
+            float out = back;
+            if (C > 1) {
+                for (int r = C - 1; r >= 0; --r) {
+                    if (r == rank) out = back;
+                    const float2 v = s_tile[par][r][plane][lane];
+                    back = fmaf(v.x, back, v.y);
+                }
+            }
+#pragma unroll
+            for (int w = W - 1; w >= 0; --w) {
+                s_out[w][plane][lane] = out;
+                out = fmaf(s_run[w][plane][lane].x, out, s_back[w][plane][lane]);
+            }
+            if (C == 1) back = out;
+        }
+        __syncthreads();
+        // f (h_{t-1} - x) of each step, then backwards through the run
+        float v[CH];
+        L q[S];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] = s_in[warp][j][lane];
+        L hs = L::of(v);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float xv[CH];
+            Word<T>::unpack(xr[s * 32], xv);
+            const L xl = L::of(xv);
+            q[s] = f[s] * fma(xl, L::of(-1.0f), hs);
+            hs = fma(f[s], hs, keep[s] * xl);
+        }
+#pragma unroll
+        for (int j = 0; j < CH; ++j) v[j] = s_out[warp][j][lane];
+        L r = L::of(v);
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+            float dv[CH], gx[CH], gg[CH];
+            Word<T>::unpack(dr[s * 32], dv);
+            r = s == S - 1 ? L::of(dv) + r : fma(f[s + 1 < S ? s + 1 : s], r, L::of(dv));
+            const L kr = keep[s] * r, gl = kr * q[s];
+            kr.get(gx);
+            gl.get(gg);
+            xr[s * 32] = Word<T>::pack(gx);
+            gr[s * 32] = Word<T>::pack(gg);
+        }
+        __syncwarp();
+        dg.store(reinterpret_cast<const uint4 *>(gr - lane), t0, len, a.T, lane);
+        dx.store(reinterpret_cast<const uint4 *>(xr - lane), t0, len, a.T, lane);
+        __syncwarp();
+    }
+    copy_wait<0>();
     if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
 }
 
@@ -573,19 +956,28 @@ int32_t check_walk(const char *what, const char *name, const Walk &w, int32_t dt
     return PB_OK;
 }
 
+// whether every row of an array starts on a 16-byte boundary
+bool wide_rows(const Walk &w, int32_t dtype) {
+    const int64_t e = 16 / (int64_t)bytes_of(dtype);
+    return !w.p || (pb::aligned16(w.p) && w.sb % e == 0 && w.st % e == 0);
+}
+
 bool words(const Walk &w, int32_t dtype) {
     return !w.p || dtype == PARPY_B200_F32 ||
            (reinterpret_cast<uintptr_t>(w.p) % 4 == 0 && w.sb % 2 == 0 && w.st % 2 == 0);
 }
 
 template <typename K>
-int32_t launch_scan(K kernel, const char *what, ScanArgs &a, int channels, int threads, int C, cudaStream_t stream) {
+int32_t launch_scan(K kernel, const char *what, ScanArgs &a, int channels, int threads, size_t smem, int C,
+                    cudaStream_t stream) {
+    if (smem) PB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     a.blocks = (a.D + channels - 1) / channels;
     const long long grid = (long long)a.B * a.blocks * C;
     PB_REQUIRE(grid <= INT_MAX, "%s: shape (%d, %d, %d) needs too many blocks", what, a.B, a.T, a.D);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -607,19 +999,26 @@ int cluster_of(const ScanArgs &a, int channels, int sms) {
     return C;
 }
 
-template <typename T, bool VEC>
+enum Access { kElements, kWords, kWide };     // how rows are read: 2 or 4 bytes a lane, or staged 16 bytes a lane
+
+template <typename T, Access ACC>
 int32_t run_forward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream) {
     constexpr int channels = 32 * Word<T>::CH;
-    return launch_scan(scan_forward<T, VEC, 16, 8>, "gated_scan", a, channels, 256, cluster_of(a, channels, dev.sm_count),
-                       stream);
+    const int C = cluster_of(a, channels, dev.sm_count);
+    if constexpr (ACC == kWide)
+        return launch_scan(scan_forward_staged<T, 16, 8, SCAN_FN>, "gated_scan", a, channels, 256, SCAN_FN * 2 * kTile * 128, C,
+                           stream);
+    return launch_scan(scan_forward<T, ACC != kElements, 16, 8>, "gated_scan", a, channels, 256, 0, C, stream);
 }
-template <typename T, bool VEC>
+template <typename T, Access ACC>
 int32_t run_backward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream) {
     constexpr int channels = 32 * Word<T>::CH;
-    return launch_scan(scan_backward<T, VEC, 8, 16>, "gated_scan_grad", a, channels, 512,
-                       cluster_of(a, channels, dev.sm_count), stream);
+    const int C = cluster_of(a, channels, dev.sm_count);
+    if constexpr (ACC == kWide)
+        return launch_scan(scan_backward_staged<T, SCAN_BS, kTile / SCAN_BS, SCAN_BN>, "gated_scan_grad", a, channels, 32 * kTile / SCAN_BS, SCAN_BN * 3 * kTile * 128,
+                           C, stream);
+    return launch_scan(scan_backward<T, ACC != kElements, 8, 16>, "gated_scan_grad", a, channels, 512, 0, C, stream);
 }
-
 template <typename T>
 int32_t run_step(const void *g, const void *x, const float *state, void *h, float *last, int64_t N, int64_t D,
                  int64_t ldg, int64_t ldx, int64_t ldh, cudaStream_t stream) {
@@ -670,11 +1069,17 @@ int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, co
     rc = pb::device_info(&dev);
     if (rc) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == PARPY_B200_F32) return run_forward<float, true>(a, dev, s);
+    const bool wide = D % (16 / (int64_t)bytes_of(dtype)) == 0 && wide_rows(a.g, dtype) && wide_rows(a.x, dtype) &&
+                      wide_rows(a.h, dtype);
     const bool vec = D % 2 == 0 && words(a.g, dtype) && words(a.x, dtype) && words(a.h, dtype);
+    if (dtype == PARPY_B200_F32) return wide ? run_forward<float, kWide>(a, dev, s) : run_forward<float, kWords>(a, dev, s);
     if (dtype == PARPY_B200_BF16)
-        return vec ? run_forward<__nv_bfloat16, true>(a, dev, s) : run_forward<__nv_bfloat16, false>(a, dev, s);
-    return vec ? run_forward<__half, true>(a, dev, s) : run_forward<__half, false>(a, dev, s);
+        return wide ? run_forward<__nv_bfloat16, kWide>(a, dev, s)
+               : vec ? run_forward<__nv_bfloat16, kWords>(a, dev, s)
+                     : run_forward<__nv_bfloat16, kElements>(a, dev, s);
+    return wide ? run_forward<__half, kWide>(a, dev, s)
+           : vec ? run_forward<__half, kWords>(a, dev, s)
+                 : run_forward<__half, kElements>(a, dev, s);
 }
 
 int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
@@ -712,12 +1117,19 @@ int32_t parpy_b200_gated_scan_grad(int32_t dtype, int64_t B, int64_t T, int64_t 
     rc = pb::device_info(&dev);
     if (rc) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == PARPY_B200_F32) return run_backward<float, true>(a, dev, s);
+    const bool wide = D % (16 / (int64_t)bytes_of(dtype)) == 0 && wide_rows(a.g, dtype) && wide_rows(a.x, dtype) &&
+                      wide_rows(a.dh, dtype) && wide_rows(a.dg, dtype) && wide_rows(a.dx, dtype);
     const bool vec = D % 2 == 0 && words(a.g, dtype) && words(a.x, dtype) && words(a.dh, dtype) &&
                      words(a.dg, dtype) && words(a.dx, dtype);
+    if (dtype == PARPY_B200_F32)
+        return wide ? run_backward<float, kWide>(a, dev, s) : run_backward<float, kWords>(a, dev, s);
     if (dtype == PARPY_B200_BF16)
-        return vec ? run_backward<__nv_bfloat16, true>(a, dev, s) : run_backward<__nv_bfloat16, false>(a, dev, s);
-    return vec ? run_backward<__half, true>(a, dev, s) : run_backward<__half, false>(a, dev, s);
+        return wide ? run_backward<__nv_bfloat16, kWide>(a, dev, s)
+               : vec ? run_backward<__nv_bfloat16, kWords>(a, dev, s)
+                     : run_backward<__nv_bfloat16, kElements>(a, dev, s);
+    return wide ? run_backward<__half, kWide>(a, dev, s)
+           : vec ? run_backward<__half, kWords>(a, dev, s)
+                 : run_backward<__half, kElements>(a, dev, s);
 }
 
 int32_t parpy_b200_gated_step(int32_t dtype, int64_t N, int64_t D, const void *g, int64_t ldg, const void *x,
