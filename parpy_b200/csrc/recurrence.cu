@@ -177,6 +177,12 @@ __device__ __forceinline__ void st_cluster_f32x2(unsigned addr, float a, float b
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
 
+// Arrival at the cluster's barrier by a warp that has written nothing the others read: no fence, which would wait for
+// the warp's stores of results.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+
 struct Walk {        // one [B, T, D] array: elements between sequences and between steps
     void *p;
     long long sb, st;
@@ -599,10 +605,10 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
     int slot = 0;
     for (int round = 0; round < rounds; ++round, t0 += stride) {
         const int par = round & 1;
-        fetch(t0 + (NST - 1) * stride);      // into the rows that the round before has written back
-        copy_wait<NST - 1>();
+        copy_wait<NST - 2>();
         __syncwarp();
         unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4;
+        const int before = slot == 0 ? (NST - 1) * 2 * kRun : slot - 2 * kRun;
         slot = slot == (NST - 1) * 2 * kRun ? 0 : slot + 2 * kRun;
         L f[S], u[S], A = L::of(1.0f), B = L::of(0.0f);
 #pragma unroll
@@ -649,10 +655,16 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
                 }
                 const unsigned at = smem_u32(&s_tile[par][rank][warp][lane]);
                 for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), ta, tb);
+                cluster_arrive();
+            } else {
+                cluster_arrive_relaxed();
             }
-            cluster_arrive();
-            cluster_wait();
         }
+        // while the exchange is under way: the round before goes out, and its rows take the inputs of a later one
+        if (round > 0) h.store(reinterpret_cast<const uint4 *>(mine_rows + before + kRun), t0 - stride, len, a.T, lane);
+        __syncwarp();
+        fetch(t0 + (NST - 1) * stride);
+        if (C > 1) cluster_wait();
         if (warp < CH) {
             float in = state;
             if (C > 1) {
@@ -684,10 +696,12 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
             xr[s * 32] = Word<T>::pack(v);
         }
         __syncwarp();
-        h.store(reinterpret_cast<const uint4 *>(xr - lane), t0, len, a.T, lane);
-        __syncwarp();
     }
     copy_wait<0>();
+    if (rounds > 0) {
+        const int last = slot == 0 ? (NST - 1) * 2 * kRun : slot - 2 * kRun;
+        h.store(reinterpret_cast<const uint4 *>(mine_rows + last + kRun), t0 - stride, len, a.T, lane);
+    }
     for (; t0 < a.T; t0 += stride) h.store(reinterpret_cast<const uint4 *>(mine_rows), t0, 0, a.T, lane);   // zeros
     if (a.last && rank == 0 && warp < CH && mine < n) a.last[(long long)b * a.D + c0 + mine] = state;
 }
@@ -730,6 +744,10 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
         copy_commit();
         fill = fill == (NST - 1) * 3 * kRun ? 0 : fill + 3 * kRun;
     };
+    auto put = [&](int at, int t) {
+        dg.store(reinterpret_cast<const uint4 *>(mine_rows + at), t, len, a.T, lane);
+        dx.store(reinterpret_cast<const uint4 *>(mine_rows + at + kRun), t, len, a.T, lane);
+    };
     // a second set of planes' warps holds the state at the start of the tile, one round ahead
     auto state_of = [&](int round) {
         const int tile = round * C + rank;
@@ -746,11 +764,11 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
     int slot = 0;
     for (int round = rounds - 1; round >= 0; --round, t0 -= stride) {
         const int par = round & 1;
-        fetch(t0 - (NST - 1) * stride);
         const float entering = stored;
         stored = state_of(round - 1);
-        copy_wait<NST - 1>();
+        copy_wait<NST - 2>();
         __syncwarp();
+        const int before = slot == 0 ? (NST - 1) * 3 * kRun : slot - 3 * kRun;
         unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4,
                        *const dr = xr + kRun / 4;
         slot = slot == (NST - 1) * 3 * kRun ? 0 : slot + 3 * kRun;
@@ -822,10 +840,16 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
                 }
                 const unsigned at = smem_u32(&s_tile[par][rank][plane][lane]);
                 for (int r = 0; r < C; ++r) st_cluster_f32x2(map_to_rank(at, r), qa, qb);
+                cluster_arrive();
+            } else {
+                cluster_arrive_relaxed();
             }
-            cluster_arrive();
-            cluster_wait();
         }
+        // while the exchange is under way: the round before goes out, and its rows take the inputs of a later one
+        if (round < rounds - 1) put(before, t0 + stride);
+        __syncwarp();
+        fetch(t0 - (NST - 1) * stride);
+        if (C > 1) cluster_wait();
         if (warp < CH) {
             float out = back;
             if (C > 1) {
@@ -872,11 +896,9 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
             gr[s * 32] = Word<T>::pack(gg);
         }
         __syncwarp();
-        dg.store(reinterpret_cast<const uint4 *>(gr - lane), t0, len, a.T, lane);
-        dx.store(reinterpret_cast<const uint4 *>(xr - lane), t0, len, a.T, lane);
-        __syncwarp();
     }
     copy_wait<0>();
+    if (rounds > 0) put(slot == 0 ? (NST - 1) * 3 * kRun : slot - 3 * kRun, t0 + stride);
     if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
 }
 
