@@ -894,11 +894,12 @@ int32_t launch_stats(const char *what, const RowArgs &a, cudaStream_t stream) {
     const int32_t rc = pb::device_info(&dev);
     if (rc) return rc;
     const long long bytes = (long long)a.M * sizeof(T);
-    const bool big = bytes >= 256 * 32;
-    const int threads = big ? 256 : 128;
+    constexpr int kBig = TOP ? 256 : 128;
+    const bool big = bytes >= kBig * 32;
+    const int threads = big ? kBig : 128;
     int C = 1;
     while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 32) C *= 2;
-    return big ? launch_row_stats<T, 256, ENT, TOP, LIST>(what, a, C, dev, stream)
+    return big ? launch_row_stats<T, kBig, ENT, TOP, LIST>(what, a, C, dev, stream)
                : launch_row_stats<T, 128, ENT, TOP, LIST>(what, a, C, dev, stream);
 }
 

@@ -19,9 +19,6 @@
 
 #include <algorithm>
 #include <climits>
-#ifdef SCAN_ENV
-#include <cstdlib>
-#endif
 
 #include "../../include/parpy_b200.h"
 #include "common.cuh"
@@ -31,21 +28,8 @@ namespace {
 
 constexpr int kTile = PARPY_B200_SCAN_TILE;   // steps per tile, and per stored state
 constexpr int kMaxRanks = 8;
-#ifndef SCAN_FB
-#define SCAN_FB 2
-#endif
-#ifndef SCAN_FN
-#define SCAN_FN 3
-#endif
-#ifndef SCAN_BB
-#define SCAN_BB 1
-#endif
-#ifndef SCAN_BN
-#define SCAN_BN 3
-#endif
-#ifndef SCAN_BS
-#define SCAN_BS 8
-#endif
+constexpr int kStages = 3;                    // rounds of inputs in shared memory in the staged kernels
+constexpr float kCap = -41.5f;                // lowest gate value that is told apart (exact in all three types)
 
 // ---- four bytes of a row: the channels of one lane ------------------------------------------------------
 template <typename T>
@@ -54,6 +38,11 @@ template <>
 struct Word<float> {
     static constexpr int CH = 1;
     __device__ static void unpack(unsigned w, float (&v)[1]) { v[0] = __uint_as_float(w); }
+    __device__ static unsigned cap(unsigned w) {        // max(v, kCap), NaN for NaN
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(kCap));
+        return __float_as_uint(r);
+    }
     __device__ static unsigned pack(const float (&v)[1]) { return __float_as_uint(v[0]); }
 };
 template <>
@@ -62,6 +51,10 @@ struct Word<__nv_bfloat16> {
     __device__ static void unpack(unsigned w, float (&v)[2]) {
         v[0] = __uint_as_float(w << 16);
         v[1] = __uint_as_float(w & 0xffff0000u);
+    }
+    __device__ static unsigned cap(unsigned w) {
+        const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162 *>(&w), __float2bfloat162_rn(kCap));
+        return *reinterpret_cast<const unsigned *>(&r);
     }
     __device__ static unsigned pack(const float (&v)[2]) {
         const __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
@@ -76,18 +69,18 @@ struct Word<__half> {
         v[0] = f.x;
         v[1] = f.y;
     }
+    __device__ static unsigned cap(unsigned w) {
+        const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(kCap));
+        return *reinterpret_cast<const unsigned *>(&r);
+    }
     __device__ static unsigned pack(const float (&v)[2]) {
         const __half2 p = __floats2half2_rn(v[0], v[1]);
         return *reinterpret_cast<const unsigned *>(&p);
     }
 };
 
-// A lane's channels within a block of 32 CH: neighbours where rows allow 4-byte access (VEC), 32 apart where they
-// start at any element.
-template <typename T, bool VEC>
-__device__ __forceinline__ int channel(int lane, int j) {
-    return VEC ? lane * Word<T>::CH + j : lane + 32 * j;
-}
+// A lane's channels within a block of 32 CH are neighbours, read as one word where rows allow 4-byte access (VEC) and one
+// by one where they start at any element.
 template <typename T, bool VEC>
 __device__ __forceinline__ unsigned load_word(const T *p, int lane, int n) {
     if constexpr (VEC) {
@@ -96,8 +89,8 @@ __device__ __forceinline__ unsigned load_word(const T *p, int lane, int n) {
             asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w) : "l"(p + lane * Word<T>::CH));
         return w;
     } else {
-        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
-        const unsigned lo = lane < n ? q[lane] : 0, hi = lane + 32 < n ? q[lane + 32] : 0;
+        const unsigned short *q = reinterpret_cast<const unsigned short *>(p) + 2 * lane;
+        const unsigned lo = 2 * lane < n ? q[0] : 0, hi = 2 * lane + 1 < n ? q[1] : 0;
         return lo | (hi << 16);
     }
 }
@@ -106,9 +99,9 @@ __device__ __forceinline__ void store_word(T *p, int lane, int n, unsigned w) {
     if constexpr (VEC) {
         if (lane * Word<T>::CH < n) __stcs(reinterpret_cast<unsigned *>(p + lane * Word<T>::CH), w);
     } else {
-        unsigned short *q = reinterpret_cast<unsigned short *>(p);
-        if (lane < n) q[lane] = (unsigned short)w;
-        if (lane + 32 < n) q[lane + 32] = (unsigned short)(w >> 16);
+        unsigned short *q = reinterpret_cast<unsigned short *>(p) + 2 * lane;
+        if (2 * lane < n) q[0] = (unsigned short)w;
+        if (2 * lane + 1 < n) q[1] = (unsigned short)(w >> 16);
     }
 }
 
@@ -155,22 +148,27 @@ __device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
 }
 
 // f = sigmoid(g) and 1 - f, each to its own relative precision: with e = exp(-g), f = 1 / (1 + e) and 1 - f = e f.
-// The exponent is capped so that e f stays 1 for g far below zero; a NaN passes.
-template <int CH>
-__device__ __forceinline__ void gate(const float (&g)[CH], Lanes<CH> &f, Lanes<CH> &keep) {
-    float t[CH], e[CH], d[CH], r[CH];
-    (Lanes<CH>::of(g) * Lanes<CH>::of(-1.4426950408889634f)).get(t);
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(t[j]) : "f"(t[j]), "f"(126.0f));
-        e[j] = pb::ex2_approx(t[j]);
-    }
-    const Lanes<CH> el = Lanes<CH>::of(e);
-    (el + Lanes<CH>::of(1.0f)).get(d);
-#pragma unroll
-    for (int j = 0; j < CH; ++j) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[j]) : "f"(d[j]));
-    f = Lanes<CH>::of(r);
-    keep = el * f;
+// Two channels share one reciprocal, f_0 = d_1 / (d_0 d_1) with d = 1 + e (the special unit takes 16 a clock and SM, and
+// two of these for every value would be half of its time). g is capped from below at -41.5, where f = 2^-60 is nothing
+// beside 1 - f = 1, so that the product stays finite; a NaN passes.
+__device__ __forceinline__ float reciprocal(float d) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return r;
+}
+__device__ __forceinline__ void gate(const float (&g)[1], Lanes<1> &f, Lanes<1> &keep) {
+    const float e = pb::ex2_approx(-1.4426950408889634f * g[0]);
+    f = Lanes<1>::of(reciprocal(1.0f + e));
+    keep = Lanes<1>::of(e) * f;
+}
+__device__ __forceinline__ void gate(const float (&g)[2], Lanes<2> &f, Lanes<2> &keep) {
+    float t[2], d[2];
+    (Lanes<2>::of(g) * Lanes<2>::of(-1.4426950408889634f)).get(t);
+    const Lanes<2> e = Lanes<2>::of(pb::ex2_approx(t[0]), pb::ex2_approx(t[1]));
+    (e + Lanes<2>::of(1.0f)).get(d);
+    const float r = reciprocal(__fmul_rn(d[0], d[1]));
+    f = Lanes<2>::of(__fmul_rn(r, d[1]), __fmul_rn(r, d[0]));
+    keep = e * f;
 }
 
 __device__ __forceinline__ void st_cluster_f32x2(unsigned addr, float a, float b) {
@@ -241,7 +239,7 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
     T *h = start_of<T>(a.h, b, c0);
 
     float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
-    const int mine = channel<T, VEC>(lane, warp);
+    const int mine = lane * CH + warp;
     if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
     if (C > 1) {          // every CTA runs before the first store into its shared memory
         cluster_arrive();
@@ -258,9 +256,9 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH];
-            Word<T>::unpack(gw[s], gv);
+            Word<T>::unpack(Word<T>::cap(gw[s]), gv);
             Word<T>::unpack(xw[s], xv);
-            gate<CH>(gv, f[s], u[s]);
+            gate(gv, f[s], u[s]);
             u[s] = u[s] * L::of(xv);
         }
         if (t0 + S > len) {           // behind the end the state is held
@@ -369,7 +367,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
     const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
     const T *g = start_of<T>(a.g, b, c0), *x = start_of<T>(a.x, b, c0), *dh = start_of<T>(a.dh, b, c0);
     T *dg = start_of<T>(a.dg, b, c0), *dx = start_of<T>(a.dx, b, c0);
-    const int plane = warp < CH ? warp : warp - CH, mine = channel<T, VEC>(lane, plane);
+    const int plane = warp < CH ? warp : warp - CH, mine = lane * CH + plane;
     const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
 
     float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
@@ -402,8 +400,8 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH];
-            Word<T>::unpack(gw[s], gv);
-            gate<CH>(gv, f[s], keep[s]);
+            Word<T>::unpack(Word<T>::cap(gw[s]), gv);
+            gate(gv, f[s], keep[s]);
             xn[s] = xw[s];
             dn[s] = dw[s];
         }
@@ -533,41 +531,56 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One array's rows of a run: row i of the run at step t + i, 128 bytes; a lane moves 16 bytes of every fourth row.
+// One array's rows of a warp's runs: 128 bytes of each step, a lane moving 16 bytes of every fourth row. `at` is the
+// lane's place in the run that comes next; a round moves it by `round` elements.
 template <typename T, int S>
 struct Rows {
-    T *p;               // this lane's place in the first row
-    long long st;
+    T *at;
+    long long four, round;
     bool in;            // the lane's channels exist
     int sub;            // its row within four
-    __device__ Rows(const Walk &w, int b, int c0, int n, int lane) {
+    __device__ Rows(const Walk &w, int b, int c0, int n, int lane, int t, int stride) {
         constexpr int E = 16 / sizeof(T);
-        p = start_of<T>(w, b, c0) + (lane & 7) * E;
-        st = w.st;
-        in = w.p && (lane & 7) * E < n;
         sub = lane >> 3;
+        at = start_of<T>(w, b, c0) + (lane & 7) * E + (t + sub) * w.st;
+        four = 4 * w.st;
+        round = stride * w.st;
+        in = w.p && (lane & 7) * E < n;
     }
-    __device__ void fetch(unsigned to, int t, int end, int lane) const {
-        const T *q = p + (t + sub) * st;
-        const int left = in ? end - t - sub : 0;
+    // `left`: steps from the run's first to the end; whole runs, which all but a sequence's last are, need no comparison
+    __device__ void fetch(unsigned to, int left) {
+        const T *q = at;
+        if (in) {
+            if (left >= S) {
 #pragma unroll
-        for (int i = 0; i < S / 4; ++i)
-            if (4 * i < left) copy16(to + i * 512 + lane * 16, q + 4 * i * st);
-    }
-    __device__ void store(const uint4 *from, int t, int len, int end, int lane) const {
-        T *q = p + (t + sub) * st;
-        const int left = in ? end - t - sub : 0;
+                for (int i = 0; i < S / 4; ++i, q += four) copy16(to + i * 512, q);
+            } else {
 #pragma unroll
-        for (int i = 0; i < S / 4; ++i)
-            if (4 * i < left) {
-                const uint4 v = from[i * 32 + lane];
-                __stcs(reinterpret_cast<uint4 *>(q + 4 * i * st), t + sub + 4 * i < len ? v : make_uint4(0, 0, 0, 0));
+                for (int i = 0; i < S / 4; ++i, q += four)
+                    if (sub + 4 * i < left) copy16(to + i * 512, q);
             }
+        }
+        at += round;
+    }
+    __device__ void store(const uint4 *from, int left, int until) {     // zeros in [left, until)
+        T *q = at;
+        if (in) {
+            if (left >= S) {
+#pragma unroll
+                for (int i = 0; i < S / 4; ++i, q += four) __stcs(reinterpret_cast<uint4 *>(q), from[i * 32]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S / 4; ++i, q += four)
+                    if (sub + 4 * i < until)
+                        __stcs(reinterpret_cast<uint4 *>(q), sub + 4 * i < left ? from[i * 32] : make_uint4(0, 0, 0, 0));
+            }
+        }
+        at += round;
     }
 };
 
 template <typename T, int S, int W, int NST>
-__global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const ScanArgs a, const int C) {
+__global__ void __launch_bounds__(W * 32, 2) scan_forward_staged(const ScanArgs a, const int C) {
     static_assert(S * W == kTile, "one stored state per tile");
     constexpr int CH = Word<T>::CH, kRun = S * 128;       // bytes of one array's run
     using L = Lanes<CH>;
@@ -579,25 +592,27 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
     const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
     const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
-    const Rows<T, S> g(a.g, b, c0, n, lane), x(a.x, b, c0, n, lane), h(a.h, b, c0, n, lane);
+    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
+    int t0 = rank * kTile + warp * S, fill = 0, ahead = t0;
+    Rows<T, S> g(a.g, b, c0, n, lane, t0, stride), x(a.x, b, c0, n, lane, t0, stride), h(a.h, b, c0, n, lane, t0, stride);
     unsigned char *const mine_rows = s_rows + warp * (NST * 2 * kRun);
-    const unsigned rows = smem_u32(mine_rows);
+    const uint4 *const lane_rows = reinterpret_cast<const uint4 *>(mine_rows) + lane;
+    const unsigned rows = smem_u32(mine_rows) + lane * 16;
 
     float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
     const int mine = lane * CH + warp;
     if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
-    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
-    int t0 = rank * kTile + warp * S, fill = 0;
-    auto fetch = [&](int t) {
-        if (t < len) {
-            g.fetch(rows + fill, t, len, lane);
-            x.fetch(rows + fill + kRun, t, len, lane);
+    auto fetch = [&]() {
+        if (ahead < len) {
+            g.fetch(rows + fill, len - ahead);
+            x.fetch(rows + fill + kRun, len - ahead);
         }
+        ahead += stride;
         copy_commit();
         fill = fill == (NST - 1) * 2 * kRun ? 0 : fill + 2 * kRun;
     };
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i) fetch(t0 + i * stride);
+    for (int i = 0; i < NST - 1; ++i) fetch();
     if (C > 1) {          // every CTA runs before the first store into its shared memory
         cluster_arrive();
         cluster_wait();
@@ -614,9 +629,9 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH];
-            Word<T>::unpack(gr[s * 32], gv);
+            Word<T>::unpack(Word<T>::cap(gr[s * 32]), gv);
             Word<T>::unpack(xr[s * 32], xv);
-            gate<CH>(gv, f[s], u[s]);
+            gate(gv, f[s], u[s]);
             u[s] = u[s] * L::of(xv);
         }
         if (t0 + S > len) {                  // behind the end the state is held
@@ -661,9 +676,9 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
             }
         }
         // while the exchange is under way: the round before goes out, and its rows take the inputs of a later one
-        if (round > 0) h.store(reinterpret_cast<const uint4 *>(mine_rows + before + kRun), t0 - stride, len, a.T, lane);
+        if (round > 0) h.store(lane_rows + (before + kRun) / 16, len - t0 + stride, a.T - t0 + stride);
         __syncwarp();
-        fetch(t0 + (NST - 1) * stride);
+        fetch();
         if (C > 1) cluster_wait();
         if (warp < CH) {
             float in = state;
@@ -700,14 +715,14 @@ __global__ void __launch_bounds__(W * 32, SCAN_FB) scan_forward_staged(const Sca
     copy_wait<0>();
     if (rounds > 0) {
         const int last = slot == 0 ? (NST - 1) * 2 * kRun : slot - 2 * kRun;
-        h.store(reinterpret_cast<const uint4 *>(mine_rows + last + kRun), t0 - stride, len, a.T, lane);
+        h.store(lane_rows + (last + kRun) / 16, len - t0 + stride, a.T - t0 + stride);
     }
-    for (; t0 < a.T; t0 += stride) h.store(reinterpret_cast<const uint4 *>(mine_rows), t0, 0, a.T, lane);   // zeros
+    for (; t0 < a.T; t0 += stride) h.store(lane_rows, 0, a.T - t0);     // behind the end
     if (a.last && rank == 0 && warp < CH && mine < n) a.last[(long long)b * a.D + c0 + mine] = state;
 }
 
 template <typename T, int S, int W, int NST>
-__global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const ScanArgs a, const int C) {
+__global__ void __launch_bounds__(W * 32) scan_backward_staged(const ScanArgs a, const int C) {
     static_assert(S * W == kTile, "one stored state per tile");
     constexpr int CH = Word<T>::CH, kRun = S * 128;
     using L = Lanes<CH>;
@@ -720,33 +735,39 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
     const int item = blockIdx.x / C, b = item / a.blocks, c0 = (item % a.blocks) * 32 * CH;
     const int n = min(a.D - c0, 32 * CH), len = length_of(a, b);
-    const Rows<T, S> g(a.g, b, c0, n, lane), x(a.x, b, c0, n, lane), dh(a.dh, b, c0, n, lane);
-    const Rows<T, S> dg(a.dg, b, c0, n, lane), dx(a.dx, b, c0, n, lane);
+    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
     unsigned char *const mine_rows = s_rows + warp * (NST * 3 * kRun);
-    const unsigned rows = smem_u32(mine_rows);
+    const uint4 *const lane_rows = reinterpret_cast<const uint4 *>(mine_rows) + lane;
+    const unsigned rows = smem_u32(mine_rows) + lane * 16;
     const int plane = warp < CH ? warp : warp - CH, mine = lane * CH + plane;
     const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
 
     float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
     if (warp < CH && a.dlast && mine < n) back = a.dlast[(long long)b * a.D + c0 + mine];
-    const int stride = C * kTile, rounds = (len + stride - 1) / stride;
-    for (int t = rounds * stride + rank * kTile + warp * S; t < a.T; t += stride) {      // behind the end
-        dg.store(reinterpret_cast<const uint4 *>(mine_rows), t, 0, a.T, lane);
-        dx.store(reinterpret_cast<const uint4 *>(mine_rows), t, 0, a.T, lane);
-    }
-    int t0 = (rounds - 1) * stride + rank * kTile + warp * S, fill = 0;
-    auto fetch = [&](int t) {
-        if (t >= 0 && t < len) {
-            g.fetch(rows + fill, t, len, lane);
-            x.fetch(rows + fill + kRun, t, len, lane);
-            dh.fetch(rows + fill + 2 * kRun, t, len, lane);
+    {
+        int t = rounds * stride + rank * kTile + warp * S;      // behind the end
+        Rows<T, S> dg(a.dg, b, c0, n, lane, t, stride), dx(a.dx, b, c0, n, lane, t, stride);
+        for (; t < a.T; t += stride) {
+            dg.store(lane_rows, 0, a.T - t);
+            dx.store(lane_rows, 0, a.T - t);
         }
+    }
+    int t0 = (rounds - 1) * stride + rank * kTile + warp * S, fill = 0, ahead = t0;
+    Rows<T, S> g(a.g, b, c0, n, lane, t0, -stride), x(a.x, b, c0, n, lane, t0, -stride), dh(a.dh, b, c0, n, lane, t0, -stride);
+    Rows<T, S> dg(a.dg, b, c0, n, lane, t0, -stride), dx(a.dx, b, c0, n, lane, t0, -stride);
+    auto fetch = [&]() {
+        if (ahead >= 0) {
+            g.fetch(rows + fill, len - ahead);
+            x.fetch(rows + fill + kRun, len - ahead);
+            dh.fetch(rows + fill + 2 * kRun, len - ahead);
+        }
+        ahead -= stride;
         copy_commit();
         fill = fill == (NST - 1) * 3 * kRun ? 0 : fill + 3 * kRun;
     };
-    auto put = [&](int at, int t) {
-        dg.store(reinterpret_cast<const uint4 *>(mine_rows + at), t, len, a.T, lane);
-        dx.store(reinterpret_cast<const uint4 *>(mine_rows + at + kRun), t, len, a.T, lane);
+    auto put = [&](int slot_at, int t) {
+        dg.store(lane_rows + slot_at / 16, len - t, a.T - t);
+        dx.store(lane_rows + (slot_at + kRun) / 16, len - t, a.T - t);
     };
     // a second set of planes' warps holds the state at the start of the tile, one round ahead
     auto state_of = [&](int round) {
@@ -756,7 +777,7 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
     };
     float stored = state_of(rounds - 1);
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i) fetch(t0 - i * stride);
+    for (int i = 0; i < NST - 1; ++i) fetch();
     if (C > 1) {
         cluster_arrive();
         cluster_wait();
@@ -772,12 +793,16 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
         unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4,
                        *const dr = xr + kRun / 4;
         slot = slot == (NST - 1) * 3 * kRun ? 0 : slot + 3 * kRun;
-        L f[S], keep[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
+        L f[S], keep[S], xl[S], dl[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            float gv[CH];
-            Word<T>::unpack(gr[s * 32], gv);
-            gate<CH>(gv, f[s], keep[s]);
+            float gv[CH], xv[CH], dv[CH];
+            Word<T>::unpack(Word<T>::cap(gr[s * 32]), gv);
+            Word<T>::unpack(xr[s * 32], xv);
+            Word<T>::unpack(dr[s * 32], dv);
+            gate(gv, f[s], keep[s]);
+            xl[s] = L::of(xv);
+            dl[s] = L::of(dv);
         }
         const bool cut = t0 + S > len;
         if (cut) {                           // behind the end: held, and no gradient
@@ -786,26 +811,21 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
                 if (t0 + s >= len) {
                     f[s] = L::of(1.0f);
                     keep[s] = L::of(0.0f);
-                    xr[s * 32] = 0;
-                    dr[s * 32] = 0;
+                    xl[s] = dl[s] = L::of(0.0f);
                 }
         }
         if (!a.dh.p) {
 #pragma unroll
-            for (int s = 0; s < S; ++s) dr[s * 32] = 0;
+            for (int s = 0; s < S; ++s) dl[s] = L::of(0.0f);
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            float xv[CH];
-            Word<T>::unpack(xr[s * 32], xv);
             A = A * f[s];
-            B = fma(f[s], B, keep[s] * L::of(xv));
+            B = fma(f[s], B, keep[s] * xl[s]);
         }
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {       // r_s = dh_s + f_{s+1} r_{s+1}
-            float dv[CH];
-            Word<T>::unpack(dr[s * 32], dv);
-            R = s == S - 1 ? L::of(dv) : fma(f[s + 1 < S ? s + 1 : s], R, L::of(dv));
+            R = s == S - 1 ? dl[s] : fma(f[s + 1 < S ? s + 1 : s], R, dl[s]);
         }
         R = f[0] * R;
         {
@@ -848,7 +868,7 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
         // while the exchange is under way: the round before goes out, and its rows take the inputs of a later one
         if (round < rounds - 1) put(before, t0 + stride);
         __syncwarp();
-        fetch(t0 - (NST - 1) * stride);
+        fetch();
         if (C > 1) cluster_wait();
         if (warp < CH) {
             float out = back;
@@ -875,20 +895,16 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
         L hs = L::of(v);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            float xv[CH];
-            Word<T>::unpack(xr[s * 32], xv);
-            const L xl = L::of(xv);
-            q[s] = f[s] * fma(xl, L::of(-1.0f), hs);
-            hs = fma(f[s], hs, keep[s] * xl);
+            q[s] = f[s] * fma(xl[s], L::of(-1.0f), hs);
+            hs = fma(f[s], hs, keep[s] * xl[s]);
         }
 #pragma unroll
         for (int j = 0; j < CH; ++j) v[j] = s_out[warp][j][lane];
         L r = L::of(v);
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
-            float dv[CH], gx[CH], gg[CH];
-            Word<T>::unpack(dr[s * 32], dv);
-            r = s == S - 1 ? L::of(dv) + r : fma(f[s + 1 < S ? s + 1 : s], r, L::of(dv));
+            float gx[CH], gg[CH];
+            r = s == S - 1 ? dl[s] + r : fma(f[s + 1 < S ? s + 1 : s], r, dl[s]);
             const L kr = keep[s] * r, gl = kr * q[s];
             kr.get(gx);
             gl.get(gg);
@@ -902,24 +918,31 @@ __global__ void __launch_bounds__(W * 32, SCAN_BB) scan_backward_staged(const Sc
     if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
 }
 
-// ---- one token for every row: 8 channels per thread where the rows allow 16-byte access, else one ------------
+// ---- one token for every row: 8 channels per thread where the rows allow 16-byte access, else 2 ----------------
+// (2, because a pair of 16-bit channels shares its reciprocal: the step then has the scan's bits.)
 template <typename T, int VN>
 __global__ void __launch_bounds__(256) scan_step(const T *g, const T *x, const float *state, T *h, float *last,
                                                  long long N, int D, long long ldg, long long ldx, long long ldh) {
-    const int per = D / VN;
+    constexpr int CH = Word<T>::CH;
+    const int per = (D + VN - 1) / VN;
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= N * per) return;
-    const long long row = i / per, at = row * D + (i % per) * VN;
+    const long long row = i / per;
     const int c = (int)(i % per) * VN;
+    const long long at = row * D + c;
     __align__(16) T gv[VN];
     __align__(16) T xv[VN];
     __align__(16) T hv[VN];
     __align__(16) float sv[VN];
     __align__(16) float lv[VN];
-    if constexpr (VN == 1) {
-        gv[0] = g[row * ldg + c];
-        xv[0] = x[row * ldx + c];
-        sv[0] = state[at];
+    if constexpr (VN == 2) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bool in = c + k < D;
+            gv[k] = in ? g[row * ldg + c + k] : (T)0.0f;
+            xv[k] = in ? x[row * ldx + c + k] : (T)0.0f;
+            sv[k] = in ? state[at + k] : 0.0f;
+        }
     } else {
         constexpr int NV = VN * sizeof(T) / 16, NS = VN / 4;
 #pragma unroll
@@ -932,16 +955,31 @@ __global__ void __launch_bounds__(256) scan_step(const T *g, const T *x, const f
             reinterpret_cast<float4 *>(sv)[k] = reinterpret_cast<const float4 *>(state + at)[k];
     }
 #pragma unroll
-    for (int k = 0; k < VN; ++k) {
-        const float gk[1] = {(float)gv[k]};
-        Lanes<1> f, keep;
-        gate<1>(gk, f, keep);
-        lv[k] = fmaf(f.v, sv[k], keep.v * (float)xv[k]);
-        hv[k] = (T)lv[k];
+    for (int k = 0; k < VN; k += CH) {
+        float gk[CH], xk[CH], sk[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            const float v = (float)gv[k + j];
+            gk[j] = v < kCap ? kCap : v;
+            xk[j] = (float)xv[k + j];
+            sk[j] = sv[k + j];
+        }
+        Lanes<CH> f, keep;
+        gate(gk, f, keep);
+        fma(f, Lanes<CH>::of(sk), keep * Lanes<CH>::of(xk)).get(sk);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            lv[k + j] = sk[j];
+            hv[k + j] = (T)sk[j];
+        }
     }
-    if constexpr (VN == 1) {
-        h[row * ldh + c] = hv[0];
-        last[at] = lv[0];
+    if constexpr (VN == 2) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (c + k < D) {
+                h[row * ldh + c + k] = hv[k];
+                last[at + k] = lv[k];
+            }
     } else {
         constexpr int NV = VN * sizeof(T) / 16, NS = VN / 4;
 #pragma unroll
@@ -1013,9 +1051,6 @@ int32_t launch_scan(K kernel, const char *what, ScanArgs &a, int channels, int t
 
 int cluster_of(const ScanArgs &a, int channels, int sms) {
     const long long blocks = (long long)a.B * ((a.D + channels - 1) / channels);
-#ifdef SCAN_ENV
-    if (getenv("SCAN_C")) return atoi(getenv("SCAN_C"));
-#endif
     int C = 1;
     while (C < kMaxRanks && blocks * C < 2LL * sms && (long long)C * kTile < a.T) C *= 2;
     return C;
@@ -1028,8 +1063,8 @@ int32_t run_forward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream)
     constexpr int channels = 32 * Word<T>::CH;
     const int C = cluster_of(a, channels, dev.sm_count);
     if constexpr (ACC == kWide)
-        return launch_scan(scan_forward_staged<T, 16, 8, SCAN_FN>, "gated_scan", a, channels, 256, SCAN_FN * 2 * kTile * 128, C,
-                           stream);
+        return launch_scan(scan_forward_staged<T, 16, 8, kStages>, "gated_scan", a, channels, 256,
+                           kStages * 2 * kTile * 128, C, stream);
     return launch_scan(scan_forward<T, ACC != kElements, 16, 8>, "gated_scan", a, channels, 256, 0, C, stream);
 }
 template <typename T, Access ACC>
@@ -1037,8 +1072,8 @@ int32_t run_backward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream
     constexpr int channels = 32 * Word<T>::CH;
     const int C = cluster_of(a, channels, dev.sm_count);
     if constexpr (ACC == kWide)
-        return launch_scan(scan_backward_staged<T, SCAN_BS, kTile / SCAN_BS, SCAN_BN>, "gated_scan_grad", a, channels, 32 * kTile / SCAN_BS, SCAN_BN * 3 * kTile * 128,
-                           C, stream);
+        return launch_scan(scan_backward_staged<T, 8, 16, kStages>, "gated_scan_grad", a, channels, 512,
+                           kStages * 3 * kTile * 128, C, stream);
     return launch_scan(scan_backward<T, ACC != kElements, 8, 16>, "gated_scan_grad", a, channels, 512, 0, C, stream);
 }
 template <typename T>
@@ -1047,11 +1082,11 @@ int32_t run_step(const void *g, const void *x, const float *state, void *h, floa
     constexpr int E = 16 / sizeof(T);
     const bool wide = D % 8 == 0 && ldg % E == 0 && ldx % E == 0 && ldh % E == 0 && pb::aligned16(g) &&
                       pb::aligned16(x) && pb::aligned16(state) && pb::aligned16(h) && pb::aligned16(last);
-    const long long work = N * (wide ? D / 8 : D), blocks = (work + 255) / 256;
+    const long long work = N * (wide ? D / 8 : (D + 1) / 2), blocks = (work + 255) / 256;
     PB_REQUIRE(blocks <= INT_MAX, "gated_step: shape (%lld, %lld) is too large", (long long)N, (long long)D);
     const T *gt = static_cast<const T *>(g), *xt = static_cast<const T *>(x);
     if (wide) scan_step<T, 8><<<(unsigned)blocks, 256, 0, stream>>>(gt, xt, state, static_cast<T *>(h), last, N, (int)D, ldg, ldx, ldh);
-    else scan_step<T, 1><<<(unsigned)blocks, 256, 0, stream>>>(gt, xt, state, static_cast<T *>(h), last, N, (int)D, ldg, ldx, ldh);
+    else scan_step<T, 2><<<(unsigned)blocks, 256, 0, stream>>>(gt, xt, state, static_cast<T *>(h), last, N, (int)D, ldg, ldx, ldh);
     PB_CUDA(cudaGetLastError());
     return PB_OK;
 }
