@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 #include <cmath>
 
 #include "../../include/parpy_b200.h"
@@ -32,8 +33,6 @@ constexpr double kLn2 = 0.693147180559945309417;
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr int kTopMax = 128;         // alternatives a row can ask for
 constexpr int kListMax = 1024;       // entries of a teacher's list
-constexpr int kCand = 1024;          // candidates of one selection round
-constexpr int kSample = 256;         // of them, where there are more, that give the next round's bound
 constexpr int kGroups = 128;         // most thread groups whose best values give the first bound
 constexpr int kMaxCluster = 8;
 
@@ -360,9 +359,11 @@ template <int THREADS, bool TOP>
 struct TopSmem {};
 template <int THREADS>
 struct TopSmem<THREADS, true> {
+    // a warp that has a row to itself is one of 32 on its SM, and never in a cluster
+    static constexpr int kCand = THREADS == 32 ? 128 : 512;
     u64 group[kGroups];
     u64 cand[kCand];
-    u64 merge[kMaxCluster * kTopMax];
+    u64 merge[THREADS == 32 ? 1 : kMaxCluster * kTopMax];
     int sel[THREADS];
     u64 tau;
     int nsel, ncand;
@@ -387,7 +388,7 @@ __device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
 // Rows dealt to clusters of C CTAs, vectors of a row round robin to the cluster's threads.
 template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowArgs a, const int C) {
-    constexpr int VE = Elem<T>::VE, NW = THREADS / 32, U = ENT ? 1 : 2;
+    constexpr int VE = Elem<T>::VE, NW = THREADS / 32, U = ENT && sizeof(T) == 2 ? 1 : 2;
     __shared__ Sums s_warp[NW];
     __shared__ Sums s_rank[kMaxCluster];
     __shared__ double s_ref, s_log;     // the row's reference value and log(S): lse = ref / temperature + log(S)
@@ -419,6 +420,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
     }
     if (C > 1) cluster_arrive();     // matched before the first store into rank 0's shared memory
 
+    int token_ahead = -1;            // of the thread that writes the results: the next row's token, M for one past the row
+    if (LIST == kNone && rank == 0 && tid == 0 && a.tokens)
+        token_ahead = (int)pb::ll_max(-1, pb::ll_min(load_index(a.tokens, blockIdx.x / C, a.wide), a.M));
   // with C > 1 every cluster has one row
   for (long long row = blockIdx.x / C; row < a.N; row += rows_apart) {
     const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
@@ -430,12 +434,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
             s_top.ncand = 0;
         }
     }
-    float x_token = 0.0f;
-    long long token = -1;
+    T x_token = Elem<T>::from_float(0.0f);
+    int token = -1;
     if constexpr (LIST == kNone) {
         if (rank == 0 && tid == 0 && a.tokens) {
-            token = load_index(a.tokens, row, a.wide);
-            if (token >= 0 && token < a.M) x_token = Elem<T>::to_float(xr[token]);
+            token = token_ahead;
+            if (token >= 0 && token < a.M) x_token = xr[token];
+            if (row + rows_apart < a.N) token_ahead = (int)pb::ll_max(-1, pb::ll_min(load_index(a.tokens, row + rows_apart, a.wide), a.M));
         }
     }
     int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
@@ -569,7 +574,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
     // well: with 64 groups and K = 20 about 24 elements pass, with 128 about 22. A vector's place stands for its
     // columns; the bound takes the vector's last column, so that it never cuts off a tie.
     u64 key = 0, group_key = 0;
-    const int groups = a.K <= 32 ? kGroups / 2 : kGroups, GL = THREADS / groups, sub = tid & (GL - 1);
+    const int sample = max(64, 2 * a.K);
+    const int groups = min(a.K <= 32 ? kGroups / 2 : kGroups, THREADS), GL = THREADS / groups, sub = tid & (GL - 1);
     if constexpr (TOP) {
         key = best_v < 0 ? 0 : key_of(best, max(rv.first(best_v), 0));
         group_key = key;
@@ -590,6 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
     int n_local = 0;
     if constexpr (TOP) {
         int above = 0;
+#pragma unroll 4
         for (int j = sub; j < groups; j += GL) above += s_top.group[j] > group_key;
         for (int o = GL >> 1; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
         if (sub == 0 && above == a.K - 1 && group_key != 0) s_top.tau = group_key - (VE - 1);
@@ -597,32 +604,33 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
         u64 tau = s_top.tau;
         if (key != 0 && key >= tau) s_top.sel[atomicAdd(&s_top.nsel, 1)] = tid;
         __syncthreads();
-        const int nsel = s_top.nsel;
+        const int nsel = s_top.nsel, per = (rv.nvec + total - 1) / total;
         while (true) {
-            for (int i = warp; i < nsel; i += NW) {      // a warp goes through the vectors of one such thread
-                const int from = rank * THREADS + s_top.sel[i];
-                for (int at = from + lane * total; at < rv.nvec; at += 32 * total) {
-                    const Vec r = rv.whole(at) ? ld_const(rv.at(at)) : rv.edge(at);
-                    const int c0 = rv.first(at);
-                    if (order_of(Elem<T>::vmax(r)) < (unsigned)(tau >> 32)) continue;
+            for (int it = tid; it < nsel * per; it += THREADS) {
+                const int s = it / per, at = rank * THREADS + s_top.sel[s] + (it - s * per) * total;
+                if (at >= rv.nvec) continue;
+                const Vec r = rv.whole(at) ? ld_const(rv.at(at)) : rv.edge(at);
+                const int c0 = rv.first(at);
+                if (order_of(Elem<T>::vmax(r)) < (unsigned)(tau >> 32)) continue;
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        const u64 k = key_of(element<T>(r, e), c0 + e);
-                        if (k >= tau && c0 + e >= 0 && c0 + e < a.M) {
-                            const int p = atomicAdd(&s_top.ncand, 1);
-                            if (p < kCand) s_top.cand[p] = k;
-                        }
+                for (int e = 0; e < VE; ++e) {
+                    const u64 k = key_of(element<T>(r, e), c0 + e);
+                    if (k >= tau && c0 + e >= 0 && c0 + e < a.M) {
+                        const int p = atomicAdd(&s_top.ncand, 1);
+                        if (p < s_top.kCand) s_top.cand[p] = k;
                     }
                 }
             }
             __syncthreads();
             n_local = s_top.ncand;
-            if (n_local <= kCand) break;
-            // more than fit: the K-th best of any kSample of them is a higher bound, which drops kSample - K at least
-            for (int i = tid; i < kSample; i += THREADS) {
+            if (n_local <= 2 * sample) break;
+            // too many to rank, or more than there is room for: the K-th best of any `sample` of them is a higher bound,
+            // which drops sample - K of them at least
+            for (int i = tid; i < sample; i += THREADS) {
                 const u64 k = s_top.cand[i];
                 int n = 0;
-                for (int j = 0; j < kSample; ++j) n += s_top.cand[j] > k;
+#pragma unroll 4
+                for (int j = 0; j < sample; ++j) n += s_top.cand[j] > k;
                 if (n == a.K - 1) s_top.tau = k;
             }
             __syncthreads();
@@ -644,6 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
             for (int i = tid; i < n_local; i += THREADS) {
                 const u64 k = s_top.cand[i];
                 int n = 0;
+#pragma unroll 4
                 for (int j = 0; j < n_local; ++j) n += s_top.cand[j] > k;
                 if (n < a.K) st_cluster_u64(map_to_rank(smem_u32(&s_top.merge[rank * a.K + n]), 0), k);
             }
@@ -685,11 +694,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
         } else if (lane == 0) {
             a.lse[row] = (float)lse;
             // from the difference to ref, so that a large common offset costs nothing
+            const float x = Elem<T>::to_float(x_token);
             if (a.logp)
-                a.logp[row] = token < 0                ? 0.0f
-                              : token >= a.M           ? NAN
-                              : x_token == -INFINITY   ? (isnan(lse) ? NAN : -INFINITY)
-                                                       : (float)(((double)x_token - (double)w.ref) * a.inv_t - (double)logS);
+                a.logp[row] = token < 0        ? 0.0f
+                              : token >= a.M   ? NAN
+                              : x == -INFINITY ? (isnan(lse) ? NAN : -INFINITY)
+                                               : (float)(((double)x - (double)w.ref) * a.inv_t - (double)logS);
             if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)((double)logS - kLn2 * (double)(w.E / w.S));
             s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
             s_log = (double)logS;
@@ -705,6 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
             const u64 k = from[i];
             if (k == 0) continue;
             int above = 0;
+#pragma unroll 4
             for (int j = 0; j < n; ++j) above += from[j] > k;
             if (above >= a.K) continue;
             const float x = value_of((unsigned)(k >> 32));
@@ -894,11 +905,16 @@ int32_t launch_stats(const char *what, const RowArgs &a, cudaStream_t stream) {
     const int32_t rc = pb::device_info(&dev);
     if (rc) return rc;
     const long long bytes = (long long)a.M * sizeof(T);
-    constexpr int kBig = TOP ? 256 : 128;
-    const bool big = bytes >= kBig * 32;
+    constexpr int kBig = TOP || LIST == kTail ? 256 : 128;
+    const bool big = bytes >= 4 * kBig * 32;
     const int threads = big ? kBig : 128;
     int C = 1;
     while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 32) C *= 2;
+    if (getenv("ROW_C")) C = atoi(getenv("ROW_C"));
+    if constexpr (LIST == kNone) {
+        // a row that gives a lane four vectors at most is one warp's (32 groups bound up to 32 alternatives)
+        if (bytes <= 4 * 32 * 32 && a.K <= 32) return launch_row_stats<T, 32, ENT, TOP, LIST>(what, a, 1, dev, stream);
+    }
     return big ? launch_row_stats<T, kBig, ENT, TOP, LIST>(what, a, C, dev, stream)
                : launch_row_stats<T, 128, ENT, TOP, LIST>(what, a, C, dev, stream);
 }
