@@ -96,26 +96,41 @@ def _stage_one(arg, role, where, staged):
     raise RuntimeError(f"Argument {where} has unsupported type {type(arg)}")
 
 
+def _as_they_are(spec, args, kwargs):
+    """Whether a call needs no staging: the backend has been found usable on the current device, the options are plain, and
+    every argument is a number, None or a CUDA tensor of this device that a buffer would wrap without a change. Such
+    calls cost the host a few microseconds less; everything else takes the long way with its checks."""
+    if len(kwargs) != 1 or len(args) != len(spec.params) or not backend._usable:
+        return False
+    opts = kwargs.get("opts")
+    if type(opts) is not CompileOptions or opts.verbose_backend_resolution or opts.backend is CompileBackend.Metal:
+        return False
+    import torch
+    from . import _native
+    from .buffer import _torch_dtypes
+    device = torch._C._cuda_getDevice()
+    if (device, _native.LIB_PATH) not in backend._usable:
+        return False
+    tensors, types, strided = torch.Tensor, _torch_dtypes(), torch.strided
+    for arg, pitched in zip(args, spec.pitched):
+        kind = type(arg)
+        if kind is tensors:
+            if arg.get_device() != device or arg.dtype not in types or arg.requires_grad or \
+                    arg.layout is not strided or not (pitched or arg.is_contiguous()):
+                return False
+        elif arg is not None and kind is not int and kind is not float and kind is not bool:
+            return False
+    opts.backend = CompileBackend.Cuda      # what resolving makes of Auto
+    return True
+
+
 def _stage_arguments(spec, args, opts):
     staged = []
     out = []
     if len(args) != len(spec.params):
         raise TypeError(f"{spec.name}() takes {len(spec.params)} positional arguments "
                         f"({', '.join(spec.params)}) but {len(args)} were given")
-    import torch
-    from .buffer import _torch_dtypes
-    device = torch.cuda.current_device() if torch.cuda.is_initialized() else None     # a host tensor says -1
-    types, strided = _torch_dtypes(), torch.strided
     for i, (name, arg) in enumerate(zip(spec.params, args)):
-        if type(arg) is torch.Tensor and arg.get_device() == device:
-            # an array that CudaBuffer would wrap as it is needs no wrapping
-            if arg.dtype in types and not arg.requires_grad and arg.layout is strided and \
-                    (arg.is_contiguous() or str(spec.roles.get(name)).endswith("_rows")):
-                out.append(arg)
-                continue
-        elif arg is None or type(arg) is int or type(arg) is float:
-            out.append(arg)
-            continue
         if isinstance(arg, dict):
             d = {}
             for k, v in arg.items():
@@ -149,6 +164,9 @@ def jit(fun):
 
     @functools.wraps(fun)
     def inner(*args, **kwargs):
+        if _as_they_are(spec, args, kwargs):
+            spec.adapter(kwargs["opts"], *args)
+            return
         opts = backend._resolve_backend(_check_kwargs(kwargs, name), True)
         dev_args, staged = _stage_arguments(spec, args, opts)
         try:

@@ -32,6 +32,7 @@ class OpSpec:
         self.roles = roles          # param -> role, or param -> {key -> role} for dict args
         self.adapter = adapter
         self.doc = doc
+        self.pitched = tuple(str(roles.get(p)).endswith("_rows") for p in self.params)
 
 
 REGISTRY = {}   # name -> [OpSpec]
