@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdlib>
 #include <cmath>
@@ -881,8 +882,12 @@ int32_t check_rows(const char *what, const void *x, int32_t dtype, int64_t ldx, 
 template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
 int32_t launch_row_stats(const char *what, const RowArgs &a, int C, const pb::DeviceInfo &dev, cudaStream_t stream) {
     auto kernel = row_stats<T, THREADS, ENT, TOP, LIST>;
-    int per_sm = 1;
-    PB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, THREADS, 0));
+    static std::atomic<int> resident{0};      // the same on every device the library runs on
+    int per_sm = resident.load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        PB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, THREADS, 0));
+        resident.store(std::max(per_sm, 1), std::memory_order_relaxed);
+    }
     // a row for each cluster, or as many CTAs as are resident, which take rows in turn
     const long long grid = C > 1 ? a.N * C : std::min<long long>(a.N, (long long)std::max(per_sm, 1) * dev.sm_count);
     PB_REQUIRE(grid <= INT_MAX, "%s: %lld rows are too many", what, a.N);

@@ -150,7 +150,8 @@ __device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
 // f = sigmoid(g) and 1 - f, each to its own relative precision: with e = exp(-g), f = 1 / (1 + e) and 1 - f = e f.
 // Two channels share one reciprocal, f_0 = d_1 / (d_0 d_1) with d = 1 + e (the special unit takes 16 a clock and SM, and
 // two of these for every value would be half of its time). g is capped from below at -41.5, where f = 2^-60 is nothing
-// beside 1 - f = 1, so that the product stays finite; a NaN passes.
+// beside 1 - f = 1, so that the product stays finite; a NaN gate, whose d the minimum leaves out of the product, stays in
+// its own channel.
 __device__ __forceinline__ float reciprocal(float d) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
@@ -166,8 +167,10 @@ __device__ __forceinline__ void gate(const float (&g)[2], Lanes<2> &f, Lanes<2> 
     (Lanes<2>::of(g) * Lanes<2>::of(-1.4426950408889634f)).get(t);
     const Lanes<2> e = Lanes<2>::of(pb::ex2_approx(t[0]), pb::ex2_approx(t[1]));
     (e + Lanes<2>::of(1.0f)).get(d);
+    d[0] = fminf(d[0], 0x1p62f);
+    d[1] = fminf(d[1], 0x1p62f);
     const float r = reciprocal(__fmul_rn(d[0], d[1]));
-    f = Lanes<2>::of(__fmul_rn(r, d[1]), __fmul_rn(r, d[0]));
+    f = fma(e, Lanes<2>::of(0.0f), Lanes<2>::of(__fmul_rn(r, d[1]), __fmul_rn(r, d[0])));
     keep = e * f;
 }
 
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
     load_run<T, VEC, S>(xw, x + t0 * a.x.st, a.x.st, len - t0, lane, n);
     for (int round = 0; round < rounds; ++round, t0 += stride) {
         const int par = round & 1;
-        L f[S], u[S], A = L::of(1.0f), B = L::of(0.0f);
+        L f[S], u[S], A, B;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH];
@@ -269,6 +272,8 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
                     u[s] = L::of(0.0f);
                 }
         }
+        A = L::of(1.0f);
+        B = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             A = A * f[s];
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
     if (rounds > 0) fetch(t0, (rounds - 1) * C + rank);
     for (int round = rounds - 1; round >= 0; --round, t0 -= stride) {
         const int par = round & 1;
-        L f[S], keep[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
+        L f[S], keep[S], A, B, R = L::of(0.0f);
         unsigned xn[S], dn[S];
         const float entering = stored;
 #pragma unroll
@@ -413,6 +418,8 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
                     keep[s] = L::of(0.0f);
                 }
         }
+        A = L::of(1.0f);
+        B = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float xv[CH];
@@ -625,7 +632,7 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward_staged(const ScanArgs 
         unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4;
         const int before = slot == 0 ? (NST - 1) * 2 * kRun : slot - 2 * kRun;
         slot = slot == (NST - 1) * 2 * kRun ? 0 : slot + 2 * kRun;
-        L f[S], u[S], A = L::of(1.0f), B = L::of(0.0f);
+        L f[S], u[S], A, B;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH];
@@ -642,6 +649,8 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward_staged(const ScanArgs 
                     u[s] = L::of(0.0f);
                 }
         }
+        A = L::of(1.0f);
+        B = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             A = A * f[s];
@@ -793,7 +802,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward_staged(const ScanArgs a,
         unsigned *const gr = reinterpret_cast<unsigned *>(mine_rows + slot) + lane, *const xr = gr + kRun / 4,
                        *const dr = xr + kRun / 4;
         slot = slot == (NST - 1) * 3 * kRun ? 0 : slot + 3 * kRun;
-        L f[S], keep[S], xl[S], dl[S], A = L::of(1.0f), B = L::of(0.0f), R = L::of(0.0f);
+        L f[S], keep[S], xl[S], dl[S], A, B, R = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             float gv[CH], xv[CH], dv[CH];
@@ -818,6 +827,8 @@ __global__ void __launch_bounds__(W * 32) scan_backward_staged(const ScanArgs a,
 #pragma unroll
             for (int s = 0; s < S; ++s) dl[s] = L::of(0.0f);
         }
+        A = L::of(1.0f);
+        B = L::of(0.0f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             A = A * f[s];

@@ -447,3 +447,51 @@ def test_native_entries_refuse_before_any_launch(native):
     assert "carry" in native.error_message()
     assert lib.parpy_b200_gated_step(0, 2, 8, 64, 8, 64, 8, 64, 64, 4, 64, None) != 0
     assert "overlap" in native.error_message()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d", [64, 33])
+def test_channels_do_not_reach_one_another(d, dtype):
+    # a NaN gate and a NaN input in one channel each, in the middle of a run; every other channel as without them
+    b, t = 2, 300
+    s = inputs(b, t, d, dtype, 8)
+    clean = run(s, None)
+    step = [torch.empty_like(s["g"][:, 0]), torch.empty(b, d, device="cuda")]
+    s["g"][0, 133, 6] = math.nan
+    s["x"][1, 20, 9] = math.nan
+    s["g"][1, 0, 11] = math.nan
+    dirty = run(s, None)
+    hit = torch.zeros(b, d, dtype=torch.bool)
+    hit[0, 6] = hit[1, 9] = hit[1, 11] = True
+    others = ~hit.cuda()
+    # a neighbour's gates may be rounded otherwise in the run of the NaN: a reciprocal of its own, 4 steps of a gate
+    rel = 2.0 ** -20 if dtype == F32 else float(torch.finfo(dtype).eps)
+    for name in ("h", "dg", "dx"):
+        keep = others[:, None].expand(b, t, d)
+        a, c = clean[name][keep].float(), dirty[name][keep].float()
+        assert torch.isfinite(c).all() and float((a - c).abs().max()) <= rel * 16
+    assert torch.isnan(dirty["h"][0, 133:, 6]).all() and torch.isfinite(dirty["h"][0, :133, 6]).all()
+    assert torch.isnan(dirty["last"][hit]).all() and torch.isfinite(dirty["last"][others]).all()
+    assert torch.isnan(dirty["dh0"][0, 6]) and torch.isfinite(dirty["dh0"][others]).all()
+    kernels.gated_step(s["g"][:, 0], s["x"][:, 0], s["h0"], b, d, step[0], step[1], opts=opts())
+    assert torch.isnan(step[1][1, 11]) and int(torch.isnan(step[1]).sum()) == 1
+
+
+@gpu
+def test_state_is_carried_in_place():
+    # chunks of a long prefill: the state buffer goes in and comes out
+    b, t, d = 2, 700, 136
+    s = inputs(b, t, d, BF16, 10)
+    whole = run(s, None)
+    state = s["h0"].clone()
+    h = torch.empty_like(s["g"])
+    for at in range(0, t, 256):      # whole tiles: the same runs, composed the same way within a call
+        n = min(256, t - at)
+        kernels.gated_scan(s["g"][:, at:at + n], s["x"][:, at:at + n], state, None, b, n, d, h[:, at:at + n], state, None,
+                           opts=opts())
+    want = define(s["g"], s["x"], s["h0"], None)
+    r = room(s["g"], t)
+    close(state, want["last"], r * want["last_size"])
+    close(h, want["h"], rounding(BF16, want["h"]) + r * want["size"])
+    assert whole["last"].shape == state.shape
