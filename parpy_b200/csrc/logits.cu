@@ -21,7 +21,6 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cstdlib>
 #include <cmath>
 
 #include "../../include/parpy_b200.h"
@@ -386,7 +385,17 @@ __device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
-// Rows dealt to clusters of C CTAs, vectors of a row round robin to the cluster's threads.
+// Rows dealt to clusters of C CTAs, vectors of a row round robin to the cluster's threads; with C = 1 as many CTAs as are
+// resident take rows in turn, and a row's first vectors and token are asked for before the row before it is joined.
+//
+// What bounds it: a 16-bit logit costs one exp2 of the special unit (16 a clock and SM: 60 us for 4096 x 65536, of the
+// 82 us that reading them takes at the measured copy rate) and 7 to 8 instructions, so memory, special unit and issue are
+// all above half; the rest is a row's end, where its CTA loads nothing. Measured: 4096 x 131072 bf16 without entropy
+// 194 us (84 % of the copy rate), 4096 x 65536 with entropy 117 us (70 %), 4096 x 131072 with entropy and 20 alternatives
+// 256 us (64 %). 128 threads a row keep more rows apart in their phases than 256 (distillation 194 against 211 us); the
+// selection's end and a tail's list are shared by 256 (257 against 300 us; 45 against 53 us). Held in registers two
+// stages deep: loads that pass through shared memory (cp.async, four stages) cost 218 instead of 209 us, in 16-byte
+// pieces of a lane's own vector 322 us; scalar arithmetic instead of packed pairs 132 instead of 120 us.
 template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowArgs a, const int C) {
     constexpr int VE = Elem<T>::VE, NW = THREADS / 32, U = ENT && sizeof(T) == 2 ? 1 : 2;
@@ -422,313 +431,311 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
     if (C > 1) cluster_arrive();     // matched before the first store into rank 0's shared memory
 
     int token_ahead = -1;            // of the thread that writes the results: the next row's token, M for one past the row
-    if (LIST == kNone && rank == 0 && tid == 0 && a.tokens)
-        token_ahead = (int)pb::ll_max(-1, pb::ll_min(load_index(a.tokens, blockIdx.x / C, a.wide), a.M));
-  // with C > 1 every cluster has one row
-  for (long long row = blockIdx.x / C; row < a.N; row += rows_apart) {
-    const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
-    const Row<T> rv(xr, a.M);
-    if constexpr (TOP) {
-        if (tid == 0) {
-            s_top.tau = 0;
-            s_top.nsel = 0;
-            s_top.ncand = 0;
+    auto look_ahead = [&](long long row) {
+        if (LIST == kNone && rank == 0 && tid == 0 && a.tokens && row < a.N)
+            token_ahead = (int)pb::ll_max(-1, pb::ll_min(load_index(a.tokens, row, a.wide), a.M));
+    };
+    look_ahead(blockIdx.x / C);
+    // with C > 1 every cluster has one row
+    for (long long row = blockIdx.x / C; row < a.N; row += rows_apart) {
+        const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
+        const Row<T> rv(xr, a.M);
+        if constexpr (TOP) {
+            if (tid == 0) {
+                s_top.tau = 0;
+                s_top.nsel = 0;
+                s_top.ncand = 0;
+            }
         }
-    }
-    T x_token = Elem<T>::from_float(0.0f);
-    int token = -1;
-    if constexpr (LIST == kNone) {
-        if (rank == 0 && tid == 0 && a.tokens) {
-            token = token_ahead;
-            if (token >= 0 && token < a.M) x_token = xr[token];
-            if (row + rows_apart < a.N) token_ahead = (int)pb::ll_max(-1, pb::ll_min(load_index(a.tokens, row + rows_apart, a.wide), a.M));
+        const int token = token_ahead;
+        T x_token = Elem<T>::from_float(0.0f);
+        if (token >= 0 && token < a.M) x_token = xr[token];
+        look_ahead(row + rows_apart);
+        int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
+        if constexpr (LIST != kNone) {
+            if constexpr (LIST == kTail) s_list.head[tid] = -1;
+            load_list(s_list.l, a, row, xr);
+            if constexpr (LIST == kTail) {
+                for (int k = tid; k < a.K; k += THREADS)
+                    if (s_list.l.used[k]) {
+                        const int owner = ((s_list.l.col[k] + rv.mis) / VE) % total;
+                        if (owner / THREADS == rank)
+                            s_list.link[k] = (short)atomicExch(&s_list.head[owner % THREADS], k);
+                    }
+                __syncthreads();
+                for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) next = min(next, (s_list.l.col[k] + rv.mis) / VE);
+            }
         }
-    }
-    int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
-    if constexpr (LIST != kNone) {
-        if constexpr (LIST == kTail) s_list.head[tid] = -1;
-        load_list(s_list.l, a, row, xr);
-        if constexpr (LIST == kTail) {
-            for (int k = tid; k < a.K; k += THREADS)
-                if (s_list.l.used[k]) {
-                    const int owner = ((s_list.l.col[k] + rv.mis) / VE) % total;
-                    if (owner / THREADS == rank)
-                        s_list.link[k] = (short)atomicExch(&s_list.head[owner % THREADS], k);
-                }
-            __syncthreads();
-            for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) next = min(next, (s_list.l.col[k] + rv.mis) / VE);
-        }
-    }
 
-    float ref = 0.0f, lim = -INFINITY, best = -INFINITY;
-    int best_v = me < rv.nvec ? me : -1;
-    u64 S2 = 0, E2 = 0;
-    const u64 c2 = pack2(c, c);
+        float ref = 0.0f, lim = -INFINITY, best = -INFINITY;
+        int best_v = me < rv.nvec ? me : -1;
+        u64 S2 = 0, E2 = 0;
+        const u64 c2 = pack2(c, c);
 
-    auto take = [&](const Vec &got, int at) {
-        Vec r = got;
-        if constexpr (LIST == kTail) {
-            if (at == next) {         // listed columns are summed apart: read as masked here
-                T *e = reinterpret_cast<T *>(r.w);
-                const unsigned fill = Elem<T>::kFill;
-                next = INT_MAX;
-                for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) {
-                    const int col = s_list.l.col[k] + rv.mis, w = col / VE;
-                    if (w == at) {
+        auto take = [&](const Vec &got, int at) {
+            Vec r = got;
+            if constexpr (LIST == kTail) {
+                if (at == next) {         // listed columns are summed apart: read as masked here
+                    T *e = reinterpret_cast<T *>(r.w);
+                    const unsigned fill = Elem<T>::kFill;
+                    next = INT_MAX;
+                    for (int k = s_list.head[tid]; k >= 0; k = s_list.link[k]) {
+                        const int col = s_list.l.col[k] + rv.mis, w = col / VE;
+                        if (w == at) {
 #pragma unroll
-                        for (int i = 0; i < VE; ++i)
-                            if (i == col % VE) e[i] = *reinterpret_cast<const T *>(&fill);
-                    } else if (w > at) {
-                        next = min(next, w);
+                            for (int i = 0; i < VE; ++i)
+                                if (i == col % VE) e[i] = *reinterpret_cast<const T *>(&fill);
+                        } else if (w > at) {
+                            next = min(next, w);
+                        }
                     }
                 }
             }
-        }
-        const float vm = Elem<T>::vmax(r);
-        if constexpr (TOP) {
-            if (vm > best) {
-                best = vm;
-                best_v = at;
+            const float vm = Elem<T>::vmax(r);
+            if constexpr (TOP) {
+                if (vm > best) {
+                    best = vm;
+                    best_v = at;
+                }
             }
-        }
-        if (vm > lim) {
-            const bool fresh = lim == -INFINITY;         // nothing summed yet: ref means nothing
-            const float sh = fresh ? 0.0f : (ref - vm) * c;
-            const float f = fresh ? 0.0f : pb::ex2_approx(sh);
-            float s0, s1;
-            unpack2(S2, s0, s1);
+            if (vm > lim) {
+                const bool fresh = lim == -INFINITY;         // nothing summed yet: ref means nothing
+                const float sh = fresh ? 0.0f : (ref - vm) * c;
+                const float f = fresh ? 0.0f : pb::ex2_approx(sh);
+                float s0, s1;
+                unpack2(S2, s0, s1);
+                if constexpr (ENT) {
+                    float e0, e1;
+                    unpack2(E2, e0, e1);
+                    const float k = fmaxf(sh, -1e30f);
+                    E2 = pack2(f * (e0 + k * s0), f * (e1 + k * s1));
+                }
+                S2 = pack2(f * s0, f * s1);
+                ref = vm;
+                lim = vm + slack;
+            }
+            const u64 nref = pack2(-ref, -ref), before = E2;
+#pragma unroll
+            for (int i = 0; i < VE / 2; ++i) {
+                float x0, x1, t0, t1;
+                Elem<T>::pair(r, i, x0, x1);
+                const u64 t = mul2(add2(pack2(x0, x1), nref), c2);
+                unpack2(t, t0, t1);
+                const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
+                S2 = add2(S2, e);
+                if constexpr (ENT) E2 = fma2(e, t, E2);
+            }
             if constexpr (ENT) {
+                // a masked column adds 0 times -inf: seen by the NaN it leaves, and added again with t kept finite
                 float e0, e1;
                 unpack2(E2, e0, e1);
-                const float k = fmaxf(sh, -1e30f);
-                E2 = pack2(f * (e0 + k * s0), f * (e1 + k * s1));
-            }
-            S2 = pack2(f * s0, f * s1);
-            ref = vm;
-            lim = vm + slack;
-        }
-        const u64 nref = pack2(-ref, -ref), before = E2;
+                if (isnan(e0 + e1)) {
+                    E2 = before;
 #pragma unroll
-        for (int i = 0; i < VE / 2; ++i) {
-            float x0, x1, t0, t1;
-            Elem<T>::pair(r, i, x0, x1);
-            const u64 t = mul2(add2(pack2(x0, x1), nref), c2);
-            unpack2(t, t0, t1);
-            const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
-            S2 = add2(S2, e);
-            if constexpr (ENT) E2 = fma2(e, t, E2);
-        }
-        if constexpr (ENT) {
-            // a masked column adds 0 times -inf: seen by the NaN it leaves, and added again with t kept finite
-            float e0, e1;
-            unpack2(E2, e0, e1);
-            if (isnan(e0 + e1)) {
-                E2 = before;
-#pragma unroll
-                for (int i = 0; i < VE / 2; ++i) {
-                    float x0, x1, t0, t1;
-                    Elem<T>::pair(r, i, x0, x1);
-                    unpack2(mul2(add2(pack2(x0, x1), nref), c2), t0, t1);
-                    const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
-                    E2 = fma2(e, pack2(fmaxf(t0, -1e30f), fmaxf(t1, -1e30f)), E2);
-                }
-            }
-        }
-    };
-    auto take_all = [&](const Vec (&r)[U], int at) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) take(r[u], at + u * total);
-    };
-    if (rv.v0 && me == 0) take(rv.edge(0), 0);
-    // at most 2^28 + 1 vectors and 2^12 threads: no sum of them leaves 32 bits
-    int v = me < rv.v0 ? me + total : me;
-    bool more = v + reach < rv.v1;
-    while (more) {                   // the next vectors are on their way while these are summed
-        int then = v + U * total;
-        more = then + reach < rv.v1;
-        if (more) load(r1, rv, then);
-        take_all(r0, v);
-        v = then;
-        if (!more) break;
-        then = v + U * total;
-        more = then + reach < rv.v1;
-        if (more) load(r0, rv, then);
-        take_all(r1, v);
-        v = then;
-    }
-    for (; v < rv.v1; v += total) take(ld_const(rv.at(v)), v);
-    if (rv.tail() && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
-
-    if (row + rows_apart < a.N) open_row(row + rows_apart);
-    Sums mine;
-    {
-        float s0, s1, e0, e1;
-        unpack2(S2, s0, s1);
-        unpack2(E2, e0, e1);
-        mine = {ref, s0 + s1, e0 + e1};
-    }
-    mine = warp_join<ENT>(mine, c);
-    if (lane == 0) s_warp[warp] = mine;
-
-    // A group's best value is one of the row's elements, so the K-th best of the groups' values bounds the K-th best
-    // element from below: only threads whose own best reaches it can hold one of the K. Few groups rank fast, many bound
-    // well: with 64 groups and K = 20 about 24 elements pass, with 128 about 22. A vector's place stands for its
-    // columns; the bound takes the vector's last column, so that it never cuts off a tie.
-    u64 key = 0, group_key = 0;
-    const int sample = max(64, 2 * a.K);
-    const int groups = min(a.K <= 32 ? kGroups / 2 : kGroups, THREADS), GL = THREADS / groups, sub = tid & (GL - 1);
-    if constexpr (TOP) {
-        key = best_v < 0 ? 0 : key_of(best, max(rv.first(best_v), 0));
-        group_key = key;
-        for (int o = GL >> 1; o > 0; o >>= 1) {
-            const u64 other = __shfl_xor_sync(0xffffffffu, group_key, o);
-            group_key = other > group_key ? other : group_key;
-        }
-        if (sub == 0) s_top.group[tid / GL] = group_key;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        Sums w = lane < NW ? s_warp[lane] : Sums{0.0f, 0.0f, 0.0f};
-        w = warp_join<ENT>(w, c);
-        if (lane == 0) s_warp[0] = w;
-        __syncwarp();
-    }
-
-    int n_local = 0;
-    if constexpr (TOP) {
-        int above = 0;
-#pragma unroll 4
-        for (int j = sub; j < groups; j += GL) above += s_top.group[j] > group_key;
-        for (int o = GL >> 1; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-        if (sub == 0 && above == a.K - 1 && group_key != 0) s_top.tau = group_key - (VE - 1);
-        __syncthreads();
-        u64 tau = s_top.tau;
-        if (key != 0 && key >= tau) s_top.sel[atomicAdd(&s_top.nsel, 1)] = tid;
-        __syncthreads();
-        const int nsel = s_top.nsel, per = (rv.nvec + total - 1) / total;
-        while (true) {
-            for (int it = tid; it < nsel * per; it += THREADS) {
-                const int s = it / per, at = rank * THREADS + s_top.sel[s] + (it - s * per) * total;
-                if (at >= rv.nvec) continue;
-                const Vec r = rv.whole(at) ? ld_const(rv.at(at)) : rv.edge(at);
-                const int c0 = rv.first(at);
-                if (order_of(Elem<T>::vmax(r)) < (unsigned)(tau >> 32)) continue;
-#pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const u64 k = key_of(element<T>(r, e), c0 + e);
-                    if (k >= tau && c0 + e >= 0 && c0 + e < a.M) {
-                        const int p = atomicAdd(&s_top.ncand, 1);
-                        if (p < s_top.kCand) s_top.cand[p] = k;
+                    for (int i = 0; i < VE / 2; ++i) {
+                        float x0, x1, t0, t1;
+                        Elem<T>::pair(r, i, x0, x1);
+                        unpack2(mul2(add2(pack2(x0, x1), nref), c2), t0, t1);
+                        const u64 e = pack2(pb::ex2_approx(t0), pb::ex2_approx(t1));
+                        E2 = fma2(e, pack2(fmaxf(t0, -1e30f), fmaxf(t1, -1e30f)), E2);
                     }
                 }
             }
-            __syncthreads();
-            n_local = s_top.ncand;
-            if (n_local <= 2 * sample) break;
-            // too many to rank, or more than there is room for: the K-th best of any `sample` of them is a higher bound,
-            // which drops sample - K of them at least
-            for (int i = tid; i < sample; i += THREADS) {
-                const u64 k = s_top.cand[i];
-                int n = 0;
-#pragma unroll 4
-                for (int j = 0; j < sample; ++j) n += s_top.cand[j] > k;
-                if (n == a.K - 1) s_top.tau = k;
-            }
-            __syncthreads();
-            tau = s_top.tau;
-            if (tid == 0) s_top.ncand = 0;
-            __syncthreads();
-        }
-    }
-
-    if (C > 1) {
-        cluster_wait();
-        if (tid == 0) {
-            const unsigned to = map_to_rank(smem_u32(&s_rank[rank]), 0);
-            st_cluster_f32(to, s_warp[0].ref);
-            st_cluster_f32(to + 4, s_warp[0].S);
-            st_cluster_f32(to + 8, s_warp[0].E);
-        }
-        if constexpr (TOP) {
-            for (int i = tid; i < n_local; i += THREADS) {
-                const u64 k = s_top.cand[i];
-                int n = 0;
-#pragma unroll 4
-                for (int j = 0; j < n_local; ++j) n += s_top.cand[j] > k;
-                if (n < a.K) st_cluster_u64(map_to_rank(smem_u32(&s_top.merge[rank * a.K + n]), 0), k);
-            }
-        }
-        cluster_arrive();
-        cluster_wait();
-        if (rank != 0) return;
-    }
-
-    if (warp == 0) {
-        Sums w = C > 1 ? (lane < C ? s_rank[lane] : Sums{0.0f, 0.0f, 0.0f}) : s_warp[0];
-        if (C > 1) w = warp_join<ENT>(w, c);
-        const float logS = logf(w.S);
-        double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + (double)logS;
-        if constexpr (LIST != kNone) {
-            const Teacher t = warp_teacher<LIST == kTail, LIST == kTail>(s_list.l, a.K, a.inv_t);
-            const double rest = lse;
-            if (LIST == kTail) lse = log_add(rest, t.listed);
-            double loss = 0.0;
-            for (int k = lane; k < a.K; k += 32)
-                if (s_list.l.used[k]) {
-                    const double logq = (double)s_list.l.v[k] - (double)t.norm;
-                    const double q = (double)expf((float)logq);
-                    const double z = (double)s_list.l.x[k] * a.inv_t;
-                    if (!(q <= 0.0)) loss += q * (logq - (z == -INFINITY ? z : z - lse));
-                }
+        };
+        auto take_all = [&](const Vec (&r)[U], int at) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-            if (lane == 0) {
-                if (LIST == kTail) {
-                    const double left = left_of(t, a.M);
-                    if (left > 0.0) loss += left * (log(left) - (rest == -INFINITY ? rest : rest - lse));
-                }
-                if (s_list.l.bad || isnan(t.mass)) loss = NAN;
-                a.loss[row] = (float)loss;
-                a.lse[row] = (float)lse;
-                if (a.rest) a.rest[row] = (float)rest;
-            }
-        } else if (lane == 0) {
-            a.lse[row] = (float)lse;
-            // from the difference to ref, so that a large common offset costs nothing
-            const float x = Elem<T>::to_float(x_token);
-            if (a.logp)
-                a.logp[row] = token < 0        ? 0.0f
-                              : token >= a.M   ? NAN
-                              : x == -INFINITY ? (isnan(lse) ? NAN : -INFINITY)
-                                               : (float)(((double)x - (double)w.ref) * a.inv_t - (double)logS);
-            if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)((double)logS - kLn2 * (double)(w.E / w.S));
-            s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
-            s_log = (double)logS;
+            for (int u = 0; u < U; ++u) take(r[u], at + u * total);
+        };
+        if (rv.v0 && me == 0) take(rv.edge(0), 0);
+        // at most 2^28 + 1 vectors and 2^12 threads: no sum of them leaves 32 bits
+        int v = me < rv.v0 ? me + total : me;
+        bool more = v + reach < rv.v1;
+        while (more) {                   // the next vectors are on their way while these are summed
+            int then = v + U * total;
+            more = then + reach < rv.v1;
+            if (more) load(r1, rv, then);
+            take_all(r0, v);
+            v = then;
+            if (!more) break;
+            then = v + U * total;
+            more = then + reach < rv.v1;
+            if (more) load(r0, rv, then);
+            take_all(r1, v);
+            v = then;
         }
-    }
-    if constexpr (TOP) {
+        for (; v < rv.v1; v += total) take(ld_const(rv.at(v)), v);
+        if (rv.tail() && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
+
+        if (row + rows_apart < a.N) open_row(row + rows_apart);
+        Sums mine;
+        {
+            float s0, s1, e0, e1;
+            unpack2(S2, s0, s1);
+            unpack2(E2, e0, e1);
+            mine = {ref, s0 + s1, e0 + e1};
+        }
+        mine = warp_join<ENT>(mine, c);
+        if (lane == 0) s_warp[warp] = mine;
+
+        // A group's best value is one of the row's elements, so the K-th best of the groups' values bounds the K-th best
+        // element from below: only threads whose own best reaches it can hold one of the K. Few groups rank fast, many bound
+        // well: with 64 groups and K = 20 about 24 elements pass, with 128 about 22. A vector's place stands for its
+        // columns; the bound takes the vector's last column, so that it never cuts off a tie.
+        u64 key = 0, group_key = 0;
+        const int sample = max(64, 2 * a.K);
+        const int groups = min(a.K <= 32 ? kGroups / 2 : kGroups, THREADS), GL = THREADS / groups, sub = tid & (GL - 1);
+        if constexpr (TOP) {
+            key = best_v < 0 ? 0 : key_of(best, max(rv.first(best_v), 0));
+            group_key = key;
+            for (int o = GL >> 1; o > 0; o >>= 1) {
+                const u64 other = __shfl_xor_sync(0xffffffffu, group_key, o);
+                group_key = other > group_key ? other : group_key;
+            }
+            if (sub == 0) s_top.group[tid / GL] = group_key;
+        }
         __syncthreads();
-        const double row_ref = s_ref, row_log = s_log;
-        const bool broken = isnan(row_ref * 0.0 + row_log);     // S = 0 (log -inf) is an empty row, not a broken one
-        const u64 *from = C > 1 ? s_top.merge : s_top.cand;
-        const int n = C > 1 ? C * a.K : n_local;
-        for (int i = tid; i < n; i += THREADS) {
-            const u64 k = from[i];
-            if (k == 0) continue;
+        if (warp == 0) {
+            Sums w = lane < NW ? s_warp[lane] : Sums{0.0f, 0.0f, 0.0f};
+            w = warp_join<ENT>(w, c);
+            if (lane == 0) s_warp[0] = w;
+            __syncwarp();
+        }
+
+        int n_local = 0;
+        if constexpr (TOP) {
             int above = 0;
 #pragma unroll 4
-            for (int j = 0; j < n; ++j) above += from[j] > k;
-            if (above >= a.K) continue;
-            const float x = value_of((unsigned)(k >> 32));
-            const long long o = row * a.K + above;
-            a.top[o] = broken ? NAN : x == -INFINITY ? x : (float)(((double)x - row_ref) * a.inv_t - row_log);
-            const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
-            if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
-            else static_cast<int *>(a.at)[o] = (int)col;
+            for (int j = sub; j < groups; j += GL) above += s_top.group[j] > group_key;
+            for (int o = GL >> 1; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+            if (sub == 0 && above == a.K - 1 && group_key != 0) s_top.tau = group_key - (VE - 1);
+            __syncthreads();
+            u64 tau = s_top.tau;
+            if (key != 0 && key >= tau) s_top.sel[atomicAdd(&s_top.nsel, 1)] = tid;
+            __syncthreads();
+            const int nsel = s_top.nsel, per = (rv.nvec + total - 1) / total;
+            while (true) {
+                for (int it = tid; it < nsel * per; it += THREADS) {
+                    const int s = it / per, at = rank * THREADS + s_top.sel[s] + (it - s * per) * total;
+                    if (at >= rv.nvec) continue;
+                    const Vec r = rv.whole(at) ? ld_const(rv.at(at)) : rv.edge(at);
+                    const int c0 = rv.first(at);
+                    if (order_of(Elem<T>::vmax(r)) < (unsigned)(tau >> 32)) continue;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        const u64 k = key_of(element<T>(r, e), c0 + e);
+                        if (k >= tau && c0 + e >= 0 && c0 + e < a.M) {
+                            const int p = atomicAdd(&s_top.ncand, 1);
+                            if (p < s_top.kCand) s_top.cand[p] = k;
+                        }
+                    }
+                }
+                __syncthreads();
+                n_local = s_top.ncand;
+                if (n_local <= 2 * sample) break;
+                // too many to rank, or more than there is room for: the K-th best of any `sample` of them is a higher bound,
+                // which drops sample - K of them at least
+                for (int i = tid; i < sample; i += THREADS) {
+                    const u64 k = s_top.cand[i];
+                    int n = 0;
+#pragma unroll 4
+                    for (int j = 0; j < sample; ++j) n += s_top.cand[j] > k;
+                    if (n == a.K - 1) s_top.tau = k;
+                }
+                __syncthreads();
+                tau = s_top.tau;
+                if (tid == 0) s_top.ncand = 0;
+                __syncthreads();
+            }
         }
+
+        if (C > 1) {
+            cluster_wait();
+            if (tid == 0) {
+                const unsigned to = map_to_rank(smem_u32(&s_rank[rank]), 0);
+                st_cluster_f32(to, s_warp[0].ref);
+                st_cluster_f32(to + 4, s_warp[0].S);
+                st_cluster_f32(to + 8, s_warp[0].E);
+            }
+            if constexpr (TOP) {
+                for (int i = tid; i < n_local; i += THREADS) {
+                    const u64 k = s_top.cand[i];
+                    int n = 0;
+#pragma unroll 4
+                    for (int j = 0; j < n_local; ++j) n += s_top.cand[j] > k;
+                    if (n < a.K) st_cluster_u64(map_to_rank(smem_u32(&s_top.merge[rank * a.K + n]), 0), k);
+                }
+            }
+            cluster_arrive();
+            cluster_wait();
+            if (rank != 0) return;
+        }
+
+        if (warp == 0) {
+            Sums w = C > 1 ? (lane < C ? s_rank[lane] : Sums{0.0f, 0.0f, 0.0f}) : s_warp[0];
+            if (C > 1) w = warp_join<ENT>(w, c);
+            const float logS = logf(w.S);
+            double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + (double)logS;
+            if constexpr (LIST != kNone) {
+                const Teacher t = warp_teacher<LIST == kTail, LIST == kTail>(s_list.l, a.K, a.inv_t);
+                const double rest = lse;
+                if (LIST == kTail) lse = log_add(rest, t.listed);
+                double loss = 0.0;
+                for (int k = lane; k < a.K; k += 32)
+                    if (s_list.l.used[k]) {
+                        const double logq = (double)s_list.l.v[k] - (double)t.norm;
+                        const double q = (double)expf((float)logq);
+                        const double z = (double)s_list.l.x[k] * a.inv_t;
+                        if (!(q <= 0.0)) loss += q * (logq - (z == -INFINITY ? z : z - lse));
+                    }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+                if (lane == 0) {
+                    if (LIST == kTail) {
+                        const double left = left_of(t, a.M);
+                        if (left > 0.0) loss += left * (log(left) - (rest == -INFINITY ? rest : rest - lse));
+                    }
+                    if (s_list.l.bad || isnan(t.mass)) loss = NAN;
+                    a.loss[row] = (float)loss;
+                    a.lse[row] = (float)lse;
+                    if (a.rest) a.rest[row] = (float)rest;
+                }
+            } else if (lane == 0) {
+                a.lse[row] = (float)lse;
+                // from the difference to ref, so that a large common offset costs nothing
+                const float x = Elem<T>::to_float(x_token);
+                if (a.logp)
+                    a.logp[row] = token < 0        ? 0.0f
+                                  : token >= a.M   ? NAN
+                                  : x == -INFINITY ? (isnan(lse) ? NAN : -INFINITY)
+                                                   : (float)(((double)x - (double)w.ref) * a.inv_t - (double)logS);
+                if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)((double)logS - kLn2 * (double)(w.E / w.S));
+                s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
+                s_log = (double)logS;
+            }
+        }
+        if constexpr (TOP) {
+            __syncthreads();
+            const double row_ref = s_ref, row_log = s_log;
+            const bool broken = isnan(row_ref * 0.0 + row_log);     // S = 0 (log -inf) is an empty row, not a broken one
+            const u64 *from = C > 1 ? s_top.merge : s_top.cand;
+            const int n = C > 1 ? C * a.K : n_local;
+            for (int i = tid; i < n; i += THREADS) {
+                const u64 k = from[i];
+                if (k == 0) continue;
+                int above = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) above += from[j] > k;
+                if (above >= a.K) continue;
+                const float x = value_of((unsigned)(k >> 32));
+                const long long o = row * a.K + above;
+                a.top[o] = broken ? NAN : x == -INFINITY ? x : (float)(((double)x - row_ref) * a.inv_t - row_log);
+                const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
+                if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
+                else static_cast<int *>(a.at)[o] = (int)col;
+            }
+        }
+        __syncthreads();     // before the next row's values come into the shared memory that this one's are read from
     }
-    __syncthreads();     // before the next row's values come into the shared memory that this one's are read from
-  }
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------
@@ -739,6 +746,9 @@ struct GradArgs {
     const float *lse, *entropy, *rest, *dlogp, *dentropy, *dloss;
 };
 
+// What bounds it: memory. One exp2, 10 instructions and 4 bytes a 16-bit logit; 4096 x 131072 bf16 in 346 us is 6.2 TB/s,
+// 95 % of the measured copy rate, 4096 x 65536 with the entropy's term in 191 us 86 %. A list's columns are written by a
+// second, short pass over what the first one wrote: to look for them within the first cost 1141 us.
 // grid.x = rows x parts; the vectors of a row are dealt round robin to the threads of its parts. Every element is
 // read and written by the same thread, so dx may be x itself (a list's logits are read before the first store only
 // within a CTA: in place needs parts = 1 there).
@@ -755,7 +765,7 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
     const T *xr = static_cast<const T *>(a.x) + row * a.ldx;
     T *dr = static_cast<T *>(g.dx) + row * g.lddx;
     const Row<T> rv(xr, a.M);
-    const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 31u) == 0;
+    const unsigned apart = (unsigned)((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 31u);
     const float c = (float)(kLog2eD * a.inv_t);
 
     // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the token's
@@ -822,8 +832,12 @@ __global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int 
             Elem<T>::set_pair(o, i, slope(x0), slope(x1));
         }
         const int c0 = rv.first(at);
-        if (whole && same) {
+        if (whole && apart == 0) {
             st_stream(dr + c0, o);
+        } else if (whole && (apart & 3u) == 0) {       // rows of x and dx at different places of 32 bytes
+            unsigned *w = reinterpret_cast<unsigned *>(dr + c0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = o.w[i];
         } else {
             const T *e = reinterpret_cast<const T *>(o.w);
 #pragma unroll

@@ -97,7 +97,7 @@ def token_logprobs(x, tokens, N, M, K, temperature, logp, lse, entropy, top_logp
 @jit
 def token_logprobs_grad(x, tokens, N, M, temperature, lse, entropy, dlogp, dentropy, dx):
     """dx[N,M] = gradient of sum(dlogp * logp + dentropy * entropy) with respect to x, in x's
-    type; dx may be x. ``dlogp`` (then ``tokens``) and ``dentropy`` (then ``entropy``) may be None.
+    type; dx may be x, and must not overlap it otherwise. ``dlogp`` (then ``tokens``) and ``dentropy`` (then ``entropy``) may be None.
     The alternatives are reported, not differentiated. A row without a finite logit gets zeros."""
 
 
@@ -114,7 +114,8 @@ def distill_topk(x, index, values, N, M, K, temperature, tail, loss, lse, rest):
 
 @jit
 def distill_topk_grad(x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
-    """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x."""
+    """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x, and must
+    not overlap it otherwise. ``lse`` and ``rest`` are what ``distill_topk`` wrote for the same arguments."""
 
 
 @jit
@@ -123,7 +124,8 @@ def gated_scan(g, x, h0, lens, B, T, D, h, last, carry):
     from the state h0[B,D] (None: zeros), in 32 bits, h rounded once to the type of x. From lens[b]
     (None: T; clamped to [0, T]) on the state is held and h is zero. ``last`` [B,D] (or None) is the final state,
     ``carry`` [B,ceil(T/SCAN_TILE),D] (or None) the states that ``gated_scan_grad`` starts from; both float32,
-    as h0. CUDA arrays g, x, h may be strided between sequences and between steps."""
+    as h0; last may be h0. CUDA arrays g, x, h may be strided between sequences and between steps.
+    Gates below -41.5 count as -41.5."""
 
 
 @jit

@@ -300,6 +300,22 @@ def test_rows_that_lie_apart_and_start_anywhere(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_into_rows_of_another_pitch(dtype):
+    n, m = 21, 1030
+    x = logits(n, m, dtype, 15).cuda()
+    tokens = torch.arange(n, device="cuda")
+    dl = torch.ones(n, device="cuda")
+    out = run_logprobs(x, tokens, 0, 1.0)
+    plain = torch.empty_like(x)
+    kernels.token_logprobs_grad(x, tokens, n, m, 1.0, out["lse"], None, dl, None, plain, opts=opts())
+    for pad, c0 in ((2, 2), (1, 1), (4, 0), (16, 8), (34, 6)):
+        wide = torch.full((n, m + pad), 7.0, dtype=dtype, device="cuda")
+        kernels.token_logprobs_grad(x, tokens, n, m, 1.0, out["lse"], None, dl, None, wide[:, c0:c0 + m], opts=opts())
+        assert torch.equal(wide[:, c0:c0 + m], plain)
+        assert bool((wide[:, :c0] == 7).all()) and bool((wide[:, c0 + m:] == 7).all())
+
+@gpu
 def test_host_arrays_and_optional_outputs():
     n, m, k = 6, 500, 3
     x = logits(n, m, F32, 1)
