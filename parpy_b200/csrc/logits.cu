@@ -452,10 +452,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
         if (token >= 0 && token < a.M) x_token = xr[token];
         look_ahead(row + rows_apart);
         int next = INT_MAX;              // tail: the next vector of this thread that holds a listed column
-        if constexpr (LIST != kNone) {
-            if constexpr (LIST == kTail) s_list.head[tid] = -1;
+        if constexpr (LIST == kTail) {
+            s_list.head[tid] = -1;
             load_list(s_list.l, a, row, xr);
-            if constexpr (LIST == kTail) {
+            {
                 for (int k = tid; k < a.K; k += THREADS)
                     if (s_list.l.used[k]) {
                         const int owner = ((s_list.l.col[k] + rv.mis) / VE) % total;
@@ -567,6 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
         if (rv.tail() && me == rv.v1 % total) take(rv.edge(rv.v1), rv.v1);
 
         if (row + rows_apart < a.N) open_row(row + rows_apart);
+        if constexpr (LIST == kRenorm) load_list(s_list.l, a, row, xr);      // needed at the end only
         Sums mine;
         {
             float s0, s1, e0, e1;
@@ -747,13 +748,13 @@ struct GradArgs {
 };
 
 // What bounds it: memory. One exp2, 10 instructions and 4 bytes a 16-bit logit; 4096 x 131072 bf16 in 346 us is 6.2 TB/s,
-// 95 % of the measured copy rate, 4096 x 65536 with the entropy's term in 191 us 86 %. A list's columns are written by a
+// 95 % of the measured copy rate, 4096 x 65536 with the entropy's term in 176 us 93 %. A list's columns are written by a
 // second, short pass over what the first one wrote: to look for them within the first cost 1141 us.
 // grid.x = rows x parts; the vectors of a row are dealt round robin to the threads of its parts. Every element is
 // read and written by the same thread, so dx may be x itself (a list's logits are read before the first store only
 // within a CTA: in place needs parts = 1 there).
 template <typename T, int THREADS, int LIST>
-__global__ void __launch_bounds__(THREADS) row_grad(const GradArgs g, const int parts) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradArgs g, const int parts) {
     constexpr int VE = Elem<T>::VE, U = 2;
     __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kRenorm> s_list;
     __shared__ Teacher s_teacher;
@@ -954,7 +955,9 @@ int32_t launch_grad(const char *what, const GradArgs &g, cudaStream_t stream) {
     const int32_t rc = pb::device_info(&dev);
     if (rc) return rc;
     const long long bytes = (long long)g.r.M * sizeof(T);
-    const bool big = bytes >= 512 * 16 * 2, in_place = g.r.x == g.dx;
+    // small CTAs keep more rows apart in their phases (8192 x 16384: 113 us with 128 threads, 190 us with 512; with a list),
+    // large ones have less of a row's constants to make (4096 x 131072: 358 and 342 us)
+    const bool big = bytes >= 192 * 1024, in_place = g.r.x == g.dx;
     const int threads = big ? 512 : 128;
     int parts = 1;
     while (!(LIST != kNone && in_place) && g.r.N * parts < 4LL * dev.sm_count &&
