@@ -117,6 +117,10 @@ __device__ __forceinline__ float element(const Vec &r, int i) {
     return i & 1 ? b : a;
 }
 
+// Rounding can take a probability a little past 1: its logarithm, and an entropy, stop at 0. A NaN stays.
+__device__ __forceinline__ float at_most_zero(double v) { return v > 0.0 ? 0.0f : (float)v; }
+__device__ __forceinline__ float at_least_zero(double v) { return v < 0.0 ? 0.0f : (float)v; }
+
 // ---- packed fp32 pairs (two lanes of one 64-bit register, one instruction each) ------------------------
 __device__ __forceinline__ u64 pack2(float a, float b) {
     u64 r;
@@ -708,8 +712,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
                     a.logp[row] = token < 0        ? 0.0f
                                   : token >= a.M   ? NAN
                                   : x == -INFINITY ? (isnan(lse) ? NAN : -INFINITY)
-                                                   : (float)(((double)x - (double)w.ref) * a.inv_t - (double)logS);
-                if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : (float)((double)logS - kLn2 * (double)(w.E / w.S));
+                                                   : at_most_zero(((double)x - (double)w.ref) * a.inv_t - (double)logS);
+                if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : at_least_zero((double)logS - kLn2 * (double)(w.E / w.S));
                 s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
                 s_log = (double)logS;
             }
@@ -729,7 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
                 if (above >= a.K) continue;
                 const float x = value_of((unsigned)(k >> 32));
                 const long long o = row * a.K + above;
-                a.top[o] = broken ? NAN : x == -INFINITY ? x : (float)(((double)x - row_ref) * a.inv_t - row_log);
+                a.top[o] = broken ? NAN : x == -INFINITY ? x : at_most_zero(((double)x - row_ref) * a.inv_t - row_log);
                 const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
                 if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
                 else static_cast<int *>(a.at)[o] = (int)col;
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
     auto slope = [&](float x) {
         const float t = fmaf(x - hi, c, -lo);
         const float e = pb::ex2_approx(t);
-        return LIST == kNone ? e * fmaf(be, fmaxf(t, -1e30f), al) : e * al;
+        return LIST == kNone ? e * fmaf(be, fmaxf(t, -1024.0f), al) : e * al;      // e = 0 long before
     };
     auto put = [&](const Vec &r, int at, bool whole) {
         Vec o;

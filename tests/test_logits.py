@@ -255,6 +255,25 @@ def test_logprobs_of_masked_and_broken_rows(m, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sharp_rows_stay_probabilities(dtype):
+    # one column holds nearly everything: log-probabilities not above 0, entropies not below, whatever rounds
+    n, m = 400, 2051
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(n, m, generator=g)
+    x[torch.arange(n), torch.randint(0, m, (n,), generator=g)] = 12.0 + 40.0 * torch.rand(n, generator=g)
+    x = x.to(dtype).cuda()
+    tokens = x.float().argmax(1)
+    for t in (1.0, 0.05):
+        out = run_logprobs(x, tokens, 3, t)
+        check_logprobs(x, tokens, 3, t, out)
+        assert float(out["logp"].max()) <= 0 and float(out["top"].max()) <= 0 and float(out["entropy"].min()) >= 0
+        dx = torch.empty_like(x)
+        big = torch.full((n,), 1e9, device="cuda")
+        kernels.token_logprobs_grad(x, tokens, n, m, t, out["lse"], out["entropy"], big, big, dx, opts=opts())
+        assert torch.isfinite(dx.float()).all()
+
+@gpu
 def test_many_candidates_for_few_places():
     # a thread's columns lie one stride apart: give every one of many threads a run of values above all others, so
     # that far more columns pass the selection's first bound than its list holds
