@@ -535,9 +535,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
 // the cluster's CTAs the long sequence would take 164 us, without the gates 176 us, without both 143 us. Loading and
 // storing 4 bytes a lane and step straight from global memory spends two thirds of the instructions on addresses (270 us,
 // and 176 + 314 us); folding all runs in every warp instead of in one warp per channel plane cost 356 us. Eight steps a
-// warp and 16 warps forward (64 registers) cost 577 us, two stages and three CTAs an SM 234 us. A cluster is as
-// large as it takes to give every SM two CTAs: more of it than that only adds exchanges (115, 139, 150, 180 us for 1, 2, 4, 8
-// CTAs on the batch of 16).
+// warp and 16 warps forward (64 registers) cost 577 us, two stages and three CTAs an SM 234 us.
 __device__ __forceinline__ void copy16(unsigned to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
@@ -1069,10 +1067,16 @@ int32_t launch_scan(K kernel, const char *what, ScanArgs &a, int channels, int t
     return PB_OK;
 }
 
-int cluster_of(const ScanArgs &a, int channels, int sms) {
+// CTAs of a cluster, which share a sequence's tiles: one where the channel blocks alone occupy two thirds of the SMs, else
+// as many as are resident at once (two an SM forward, one backward). An exchange a round costs more than idle SMs or
+// a second wave: bf16, 2048 channels, 2000 steps a sequence, for 1 / 2 / 4 / 8 CTAs a cluster, forward 29 / 33 / 35 / 41 us at 128
+// blocks, 49 / 41 / 33 / 37 at 64 (twice the steps), 90 / 72 / 41 / 33 at 32 (four times); backward 45 / 70 / 78 / 98,
+// 82 / 68 / 72 / 94 and 156 / 119 / 68 / 100 us.
+int cluster_of(const ScanArgs &a, int channels, int sms, int per_sm) {
     const long long blocks = (long long)a.B * ((a.D + channels - 1) / channels);
     int C = 1;
-    while (C < kMaxRanks && blocks * C < 2LL * sms && (long long)C * kTile < a.T) C *= 2;
+    if (3 * blocks < 2LL * sms)
+        while (C < kMaxRanks && 2 * C * blocks <= (long long)per_sm * sms && (long long)C * kTile < a.T) C *= 2;
     return C;
 }
 
@@ -1081,7 +1085,7 @@ enum Access { kElements, kWords, kWide };     // how rows are read: 2 or 4 bytes
 template <typename T, Access ACC>
 int32_t run_forward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream) {
     constexpr int channels = 32 * Word<T>::CH;
-    const int C = cluster_of(a, channels, dev.sm_count);
+    const int C = cluster_of(a, channels, dev.sm_count, 2);
     if constexpr (ACC == kWide)
         return launch_scan(scan_forward_staged<T, 16, 8, kStages>, "gated_scan", a, channels, 256,
                            kStages * 2 * kTile * 128, C, stream);
@@ -1090,7 +1094,7 @@ int32_t run_forward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream)
 template <typename T, Access ACC>
 int32_t run_backward(ScanArgs &a, const pb::DeviceInfo &dev, cudaStream_t stream) {
     constexpr int channels = 32 * Word<T>::CH;
-    const int C = cluster_of(a, channels, dev.sm_count);
+    const int C = cluster_of(a, channels, dev.sm_count, 1);
     if constexpr (ACC == kWide)
         return launch_scan(scan_backward_staged<T, 8, 16, kStages>, "gated_scan_grad", a, channels, 512,
                            kStages * 3 * kTile * 128, C, stream);
