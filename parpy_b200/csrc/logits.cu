@@ -722,8 +722,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
             __syncthreads();
             const double row_ref = s_ref, row_log = s_log;
             const bool broken = isnan(row_ref * 0.0 + row_log);     // S = 0 (log -inf) is an empty row, not a broken one
+            auto put = [&](int place, float logp, long long column) {
+                const long long o = row * a.K + place;
+                a.top[o] = logp;
+                if (a.at_wide) static_cast<long long *>(a.at)[o] = column;
+                else static_cast<int *>(a.at)[o] = (int)column;
+            };
             const u64 *from = C > 1 ? s_top.merge : s_top.cand;
-            const int n = C > 1 ? C * a.K : n_local;
+            const int n = broken ? 0 : C > 1 ? C * a.K : n_local;
+            if (broken)          // a NaN may stand anywhere in the order, and fewer than K may have passed
+                for (int i = tid; i < a.K; i += THREADS) put(i, NAN, -1);
             for (int i = tid; i < n; i += THREADS) {
                 const u64 k = from[i];
                 if (k == 0) continue;
@@ -732,11 +740,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
                 for (int j = 0; j < n; ++j) above += from[j] > k;
                 if (above >= a.K) continue;
                 const float x = value_of((unsigned)(k >> 32));
-                const long long o = row * a.K + above;
-                a.top[o] = broken ? NAN : x == -INFINITY ? x : at_most_zero(((double)x - row_ref) * a.inv_t - row_log);
-                const long long col = broken ? -1 : (long long)(0xffffffffu - (unsigned)k);
-                if (a.at_wide) static_cast<long long *>(a.at)[o] = col;
-                else static_cast<int *>(a.at)[o] = (int)col;
+                put(above, x == -INFINITY ? x : at_most_zero(((double)x - row_ref) * a.inv_t - row_log),
+                    (long long)(0xffffffffu - (unsigned)k));
             }
         }
         __syncthreads();     // before the next row's values come into the shared memory that this one's are read from

@@ -273,6 +273,28 @@ def test_sharp_rows_stay_probabilities(dtype):
         kernels.token_logprobs_grad(x, tokens, n, m, t, out["lse"], out["entropy"], big, big, dx, opts=opts())
         assert torch.isfinite(dx.float()).all()
 
+
+@gpu
+@pytest.mark.parametrize("m", [24, 1000, 70001])
+def test_broken_rows_report_every_alternative_as_none(m):
+    # NaN of either sign, one or everywhere, and an infinity: NaN and -1 in all K places, the other rows as they are
+    x = torch.randn(6, m, generator=torch.Generator().manual_seed(m))
+    nan = torch.tensor([0xffc00000 - (1 << 32), 0x7fc00000], dtype=torch.int32).view(F32)
+    x[1] = nan[0]
+    x[2] = nan[1]
+    x[3, m // 2] = nan[0]
+    x[4, ::2] = nan[0]
+    x[5, 3] = INF
+    tokens = torch.zeros(6, dtype=torch.int64, device="cuda")
+    for dtype in (F32, BF16, F16):
+        xd = x.to(dtype).cuda()
+        for k in (1, 20, min(m, 24)):
+            out = run_logprobs(xd, tokens, k, 1.0)
+            assert bool((out["at"][1:] == -1).all()) and torch.isnan(out["top"][1:]).all()
+            assert torch.isnan(out["lse"][1:]).all() and torch.isnan(out["entropy"][1:]).all()
+            check_logprobs(xd[:1], tokens[:1], k, 1.0, {name: v[:1] for name, v in out.items()})
+
+
 @gpu
 def test_many_candidates_for_few_places():
     # a thread's columns lie one stride apart: give every one of many threads a run of values above all others, so
