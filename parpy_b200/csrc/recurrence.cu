@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward(const ScanArgs a, cons
     const T *g = start_of<T>(a.g, b, c0), *x = start_of<T>(a.x, b, c0);
     T *h = start_of<T>(a.h, b, c0);
 
-    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
+    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this turn
     const int mine = lane * CH + warp;
     if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
     if (C > 1) {          // every CTA runs before the first store into its shared memory
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
     const int plane = warp < CH ? warp : warp - CH, mine = lane * CH + plane;
     const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
 
-    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
+    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this turn from behind
     if (warp < CH && a.dlast && mine < n) back = a.dlast[(long long)b * a.D + c0 + mine];
     if (C > 1) {
         cluster_arrive();
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(W * 32, 2) scan_forward_staged(const ScanArgs 
     const uint4 *const lane_rows = reinterpret_cast<const uint4 *>(mine_rows) + lane;
     const unsigned rows = smem_u32(mine_rows) + lane * 16;
 
-    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this round
+    float state = 0.0f;   // of a plane's warp: entering the cluster's tiles of this turn
     const int mine = lane * CH + warp;
     if (warp < CH && a.h0 && mine < n) state = a.h0[(long long)b * a.D + c0 + mine];
     auto fetch = [&]() {
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward_staged(const ScanArgs a,
     const int plane = warp < CH ? warp : warp - CH, mine = lane * CH + plane;
     const float *carry = a.carry + (long long)b * ((a.T + kTile - 1) / kTile) * a.D + c0 + mine;
 
-    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this round from behind
+    float back = 0.0f;    // of a plane's warp: c entering the cluster's tiles of this turn from behind
     if (warp < CH && a.dlast && mine < n) back = a.dlast[(long long)b * a.D + c0 + mine];
     {
         int t = rounds * stride + rank * kTile + warp * S;      // behind the end
