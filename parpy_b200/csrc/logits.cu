@@ -939,7 +939,6 @@ int32_t launch_stats(const char *what, const RowArgs &a, cudaStream_t stream) {
     const int threads = big ? kBig : 128;
     int C = 1;
     while (C < kMaxCluster && a.N * C < 2LL * dev.sm_count && bytes / (2 * C) >= (long long)threads * 32) C *= 2;
-    if (getenv("ROW_C")) C = atoi(getenv("ROW_C"));
     if constexpr (LIST == kNone) {
         // a row that gives a lane four vectors at most is one warp's (32 groups bound up to 32 alternatives)
         if (bytes <= 4 * 32 * 32 && a.K <= 32) return launch_row_stats<T, 32, ENT, TOP, LIST>(what, a, 1, dev, stream);

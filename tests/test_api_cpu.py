@@ -216,3 +216,20 @@ def test_buffer_module_without_a_device():
         parpy.buffer.from_array(np.ndarray((10,), dtype=np.float32), 5)
     with pytest.raises(RuntimeError, match="Metal"):
         parpy.buffer.from_array(a, parpy.CompileBackend.Metal)
+
+
+def test_kernels_read_only_prefixed_environment_names():
+    # a launch takes nothing from the environment but the documented PARPY_B200_* switches, and the operators of
+    # language models take nothing at all: every check of their arguments happens before the launch
+    import re
+    csrc = os.path.join(os.path.dirname(parpy.__file__), "csrc")
+    names = {}
+    for file in sorted(os.listdir(csrc)):
+        if file.endswith((".cu", ".cuh")):
+            text = open(os.path.join(csrc, file)).read()
+            names[file] = re.findall(r"getenv\(([^)]*)\)", text)
+    assert not names["logits.cu"] and not names["recurrence.cu"]
+    for file, found in names.items():
+        for argument in found:
+            quoted = re.findall(r'"([^"]*)"', argument)
+            assert quoted and all(name.startswith("PARPY_B200_") for name in quoted), (file, argument)
