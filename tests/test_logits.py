@@ -655,3 +655,84 @@ def test_native_entries_refuse_before_any_launch(native):
     assert "element type" in native.error_message()
     assert lib.parpy_b200_distill_topk(64, 0, 8, 3, 8, 64, 1, 64, 0, 2, 1.0, 1, 64, 64, None, None) != 0
     assert "null" in native.error_message()
+
+
+# ---- rows that a CTA takes after its first -----------------------------------------------------------------
+# As many CTAs as are resident take rows in turn: at most 32 warps an SM, 148 SMs, so 4736 rows of one warp, 1184 of 128
+# threads and 592 of 256 are in flight at once. Every test below has more rows than that, rows that start at every
+# alignment, and tokens, lists and masks of each row's own.
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,m,k,entropy", [(5000, 61, 3, True), (5000, 300, 0, True), (2600, 2101, 0, True),
+                                           (2600, 3001, 0, False), (1300, 2101, 7, True), (1300, 9001, 20, True),
+                                           (700, 40009, 20, True), (700, 17003, 128, False)])
+def test_logprobs_of_more_rows_than_ctas(n, m, k, entropy, dtype):
+    x = logits(n, m, dtype, n + m + k)
+    x += (torch.arange(n) % 23 - 11).to(dtype)[:, None]     # each row its own reference
+    x[3::16] = torch.where(torch.arange(m) % 8 == 5, x[3::16], torch.full((), -INF, dtype=dtype))
+    x[n - 40::9] = -INF
+    x[n - 39::9, m // 2] = math.nan
+    tokens = torch.arange(n) * 37 % m
+    tokens[5::11] = -1
+    tokens[n - 30] = m
+    xd, td = x.cuda(), tokens.cuda()
+    out = run_logprobs(xd, td, k, 0.7, entropy=entropy)
+    d = check_logprobs(xd, td, k, 0.7, out)
+    if entropy and k == 0:
+        dl, de = torch.linspace(-2, 2, n).cuda(), torch.linspace(1, -1, n).cuda()
+        dx = torch.full_like(xd, 7.0)
+        kernels.token_logprobs_grad(xd, td, n, m, 0.7, out["lse"], out["entropy"], dl, de, dx, opts=opts())
+        want = define_logprobs_grad(d, td, dl, de, 0.7)
+        p, surprise = d["p"].nan_to_num(0), d["logps"].abs().clamp(max=200.0).nan_to_num(0)
+        size = p * (dl.cpu().abs()[:, None] + de.cpu().abs()[:, None] * (surprise + d["entropy"].nan_to_num(0)[:, None]))
+        finite = torch.where(torch.isfinite(d["lse"]), d["lse"].abs(), torch.zeros_like(d["lse"]))
+        rel = room(xd, 0.7) + 3 * H * finite[:, None] + 4 * H * surprise
+        off = p * de.cpu().abs()[:, None] * (room(xd, 0.7) * 20 + H * 400)
+        close(dx, want, rounding(dtype, want.nan_to_num(0)) + (size * rel + off) / 0.7 +
+              dl.cpu().abs()[:, None] * 2 * H / 0.7)
+
+
+def distill_rows(x, index, values, t, tail):
+    """``define_distill`` without a gradient, for lists of distinct columns: all rows at once."""
+    z = x.double().cpu() / t
+    used = index >= 0
+    v = torch.where(used, values.double(), torch.full((), -INF, dtype=torch.float64))
+    q = torch.exp(v) if tail else torch.softmax(v, 1)
+    lse = logsumexp(z)
+    lp = z.gather(1, index.clamp(min=0)) - lse[:, None]
+    loss = torch.where(q > 0, q * (torch.log(q) - lp), torch.zeros_like(q)).sum(1)
+    spot = torch.where(used, index, torch.full_like(index, z.shape[1]))
+    mask = torch.zeros(z.shape[0], z.shape[1] + 1, dtype=torch.bool).scatter_(1, spot, True)[:, :-1]
+    rest = logsumexp(z.masked_fill(mask, -INF))
+    if tail:
+        left = 1.0 - q.sum(1)
+        loss += left * (torch.log(left) - (rest - lse))
+    return loss, lse, rest
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,m,k,tail", [(2600, 3001, 20, False), (2600, 1999, 33, True), (1300, 9001, 20, True),
+                                        (1300, 17003, 64, False)])
+def test_distill_of_more_rows_than_ctas(n, m, k, tail, dtype):
+    x = logits(n, m, dtype, n + m)
+    x += (torch.arange(n) % 23 - 11).to(dtype)[:, None]
+    start, step = torch.arange(n)[:, None] * 131 % m, torch.arange(n)[:, None] % (m // k - 1) + 1
+    index = (start + step * torch.arange(k)) % m                  # distinct columns, another list in every row
+    g = torch.Generator().manual_seed(k)
+    values = torch.log_softmax(torch.randn(n, k, generator=g) * 2, 1) - 0.1
+    index[7::13, k // 2:] = -1
+    dloss = torch.linspace(-1, 1, n).cuda()
+    xd = x.cuda()
+    out = run_distill(xd, index.cuda(), values.cuda(), 0.7, tail, dloss)
+    loss, lse, rest = distill_rows(x, index, values, 0.7, tail)
+    r = room(xd, 0.7)
+    big = 40.0 + lse.abs() + x.double().abs().amax(1) / 0.7
+    close(out["lse"], lse, r + 3 * H * lse.abs())
+    close(out["loss"], loss, r + 8 * H * big + 4 * H * loss.abs())
+    if tail:
+        close(out["rest"], rest, r + 3 * H * rest.abs())
+    # the gradient's rows have a CTA each: a sample of them against the definition
+    rows = torch.arange(0, n, n // 40)
+    sub = {name: (v[rows.cuda()] if v is not None else None) for name, v in out.items()}
+    check_distill(xd[rows.cuda()], index[rows], values[rows], 0.7, tail, dloss.cpu()[rows], sub)
