@@ -495,3 +495,39 @@ def test_state_is_carried_in_place():
     close(state, want["last"], r * want["last_size"])
     close(h, want["h"], rounding(BF16, want["h"]) + r * want["size"])
     assert whole["last"].shape == state.shape
+
+
+# ---- many rounds: the staged kernels' ring of three rounds of inputs goes round several times ----------------------
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("b,t,d", [(70, 900, 128), (1, 9000, 64), (40, 1500, 256), (4, 5000, 72), (3, 2500, 520)])
+def test_many_rounds_of_staged_rows(b, t, d, dtype):
+    s = inputs(b, t, d, dtype, b + t + d)
+    check(s, None, run(s, None))
+    # ends in every slot of the ring, at and beside the ends of runs, tiles and rounds
+    ends = torch.tensor([t, 0, 1, 128 * 5, 128 * 6 + 1, 128 * 4 - 1, t - 1, 7 * 16, 640 + 17, t - 130, 3 * 128 + 8])
+    lens = ends[torch.arange(b) % len(ends)].cuda()
+    out = run(s, lens)
+    check(s, lens, out)
+    for i, n in enumerate(lens.tolist()):
+        for name in ("h", "dg", "dx"):
+            assert not out[name][i, n:].any()
+    check(s, lens, run(s, lens, h0=False, dh=False), h0=False, dh=False)
+    check(s, lens, run(s, lens, dlast=False), dlast=False)
+
+
+@gpu
+def test_chunks_give_the_whole_sequence():
+    # a prefill in chunks with the state in place against one call: each is within its bound of the definition
+    b, t, d = 2, 900, 136
+    s = inputs(b, t, d, F32, 14)
+    whole = run(s, None)
+    state, h = s["h0"].clone(), torch.empty_like(s["g"])
+    for at in range(0, t, 250):
+        n = min(250, t - at)
+        kernels.gated_scan(s["g"][:, at:at + n], s["x"][:, at:at + n], state, None, b, n, d, h[:, at:at + n], state, None,
+                           opts=opts())
+    want = define(s["g"], s["x"], s["h0"], None)
+    r = room(s["g"], t)
+    close(state, whole["last"], 2 * r * want["last_size"])
+    close(h, whole["h"], 2 * (rounding(F32, want["h"]) + r * want["size"]))
