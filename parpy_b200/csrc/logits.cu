@@ -341,7 +341,8 @@ __device__ Teacher warp_teacher(const List &l, int K, double inv_t) {
     t.any = n;
     t.norm = TAIL || sv == 0.0 ? 0.0f : vref + (float)log(sv);    // no entry with mass: every q is exp(-inf) = 0
     t.mass = !isfinite(sv) ? (double)NAN : TAIL ? sv : sv == 0.0 ? 0.0 : 1.0;
-    t.listed = !STUDENT || sx == 0.0 ? -INFINITY : (double)xref * inv_t + log(sx);
+    // a sum that is not finite holds a NaN or +inf (finite columns are taken relative to their largest): the row is broken
+    t.listed = !STUDENT || sx == 0.0 ? -INFINITY : isfinite(sx) ? (double)xref * inv_t + log(sx) : NAN;
     return t;
 }
 
@@ -699,7 +700,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
                         const double left = left_of(t, a.M);
                         if (left > 0.0) loss += left * (log(left) - (rest == -INFINITY ? rest : rest - lse));
                     }
-                    if (s_list.l.bad || isnan(t.mass)) loss = NAN;
+                    if (s_list.l.bad || isnan(t.mass) || isnan(lse)) loss = NAN;
                     a.loss[row] = (float)loss;
                     a.lse[row] = (float)lse;
                     if (a.rest) a.rest[row] = (float)rest;

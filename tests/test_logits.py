@@ -736,3 +736,35 @@ def test_distill_of_more_rows_than_ctas(n, m, k, tail, dtype):
     rows = torch.arange(0, n, n // 40)
     sub = {name: (v[rows.cuda()] if v is not None else None) for name, v in out.items()}
     check_distill(xd[rows.cuda()], index[rows], values[rows], 0.7, tail, dloss.cpu()[rows], sub)
+
+
+# ---- broken rows of a distillation -----------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("m", [24, 9001])
+def test_distill_rows_with_an_infinity_or_nan_are_nan(m, tail):
+    # +inf or NaN in a listed column while nothing else is left, under a teacher that wants that column or does not,
+    # and in a column that is not listed while the teacher wants columns which the student has masked
+    n, k = 8, 4
+    x = torch.full((n, m), -INF)
+    index = (torch.arange(k) * 3 + torch.arange(n)[:, None]) % m
+    values = torch.log(torch.tensor([0.4, 0.3, 0.2, 0.05])).repeat(n, 1)
+    x[0, index[0]] = torch.tensor([1.0, INF, 0.5, 2.0])
+    x[1, index[1]] = torch.tensor([1.0, INF, 0.5, 2.0])
+    values[1, 1] = -INF                          # the teacher has no use for it
+    x[2, index[2]] = torch.tensor([1.0, math.nan, 0.5, 2.0])
+    values[2, 1] = -INF
+    x[3, index[3, 0]] = INF
+    values[3, 0] = -INF
+    x[4] = 0.0
+    x[4, index[4]] = -INF
+    x[4, m - 1] = math.nan
+    x[5] = 0.0
+    x[5, 5] = INF
+    index[5] = -1                                # nothing listed
+    x[6] = 0.0                                   # sound
+    x[7, index[7]] = 1.0                         # sound: nothing outside the list
+    out = run_distill(x.cuda(), index.cuda(), values.cuda(), 1.0, tail, torch.ones(n).cuda())
+    for name in ("loss", "lse"):
+        assert torch.isnan(out[name][:6]).all() and not torch.isnan(out[name][6:]).any(), name
+    assert torch.isnan(out["dx"][:6]).all() and not torch.isnan(out["dx"][6:]).any()
