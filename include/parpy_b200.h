@@ -342,7 +342,7 @@ int32_t parpy_b200_viterbi_wait_probe(int32_t polls, void *stream);
  * temperature in [1e-4, 1e4]. A logit of -inf is a column that a mask took out. Sums are kept in
  * 32 bits, each output is rounded once. A row that holds a NaN or +inf gets NaN outputs
  * (top_index -1); a row without a finite logit has lse -inf, logp -inf and a zero
- * gradient. Token and column numbers are 64-bit where the wide_ flag is set, else 32-bit. */
+ * gradient. lse and rest of a row with one are finite: they stop at the range of a float. Token and column numbers are 64-bit where the wide_ flag is set, else 32-bit. */
 #define PARPY_B200_F32 0
 #define PARPY_B200_BF16 1
 #define PARPY_B200_F16 2

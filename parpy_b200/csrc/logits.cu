@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -303,11 +304,35 @@ __device__ void load_list(List &l, const RowArgs &a, long long row, const T *xr)
     __syncthreads();
 }
 
-// What one warp derives from a list: the teacher's normaliser and mass, the student's listed log-mass (natural logs).
+// The logarithm of a sum of exp(z) over some columns, as its reference logit and what is left: ref / temperature + log. A
+// logit is compared with it through the difference to ref, so that a row's common offset (a mask of the type's lowest value
+// over every column has 3.4e38) costs nothing. log = -inf: no column.
+struct Mass {
+    double ref, log;
+    __device__ double value(double inv_t) const { return log == -INFINITY ? log : ref * inv_t + log; }
+    // log of exp(x / temperature) relative to the sum
+    __device__ double below(float x, double inv_t) const {
+        return x == -INFINITY ? (double)x : ((double)x - ref) * inv_t - log;
+    }
+};
+__device__ __forceinline__ Mass join_mass(const Mass &a, const Mass &b, double inv_t) {
+    if (a.log == -INFINITY) return b;
+    if (b.log == -INFINITY) return a;
+    const double ref = fmax(a.ref, b.ref), la = (a.ref - ref) * inv_t + a.log, lb = (b.ref - ref) * inv_t + b.log;
+    const double m = fmax(la, lb);
+    return {ref, m + log(exp(la - m) + exp(lb - m))};     // NaN stays NaN
+}
+// The 32-bit output of a sum that exists is finite: it stops at the type's range. A NaN stays.
+__device__ __forceinline__ float limited(double v) {
+    const float f = (float)v;
+    return isinf(f) && !isinf(v) ? copysignf(FLT_MAX, f) : f;
+}
+
+// What one warp derives from a list: the teacher's normaliser and mass, the student's listed sum (natural logs).
 struct Teacher {
     float norm;       // q_k = exp(v_k - norm)
     double mass;      // sum q (before `left`), in 64 bits: 1 - mass is next to a border
-    double listed;    // log sum over the listed columns exp(z)
+    Mass listed;      // log sum over the listed columns exp(z)
     int any;          // entries in use
 };
 
@@ -342,15 +367,8 @@ __device__ Teacher warp_teacher(const List &l, int K, double inv_t) {
     t.norm = TAIL || sv == 0.0 ? 0.0f : vref + (float)log(sv);    // no entry with mass: every q is exp(-inf) = 0
     t.mass = !isfinite(sv) ? (double)NAN : TAIL ? sv : sv == 0.0 ? 0.0 : 1.0;
     // a sum that is not finite holds a NaN or +inf (finite columns are taken relative to their largest): the row is broken
-    t.listed = !STUDENT || sx == 0.0 ? -INFINITY : isfinite(sx) ? (double)xref * inv_t + log(sx) : NAN;
+    t.listed = {(double)xref, !STUDENT || sx == 0.0 ? -INFINITY : isfinite(sx) ? log(sx) : NAN};
     return t;
-}
-
-__device__ __forceinline__ double log_add(double a, double b) {
-    if (a == -INFINITY) return b;
-    if (b == -INFINITY) return a;
-    const double m = fmax(a, b);
-    return m + log(exp(a - m) + exp(b - m));     // NaN stays NaN
 }
 
 // mass of the bucket of all other columns: none where every column is listed
@@ -679,41 +697,41 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
         if (warp == 0) {
             Sums w = C > 1 ? (lane < C ? s_rank[lane] : Sums{0.0f, 0.0f, 0.0f}) : s_warp[0];
             if (C > 1) w = warp_join<ENT>(w, c);
-            const float logS = logf(w.S);
-            double lse = w.S == 0.0f ? -INFINITY : (double)w.ref * a.inv_t + (double)logS;
+            const float logS = logf(w.S);       // -inf for 0
+            const Mass rest{(double)w.ref, (double)logS};
             if constexpr (LIST != kNone) {
                 const Teacher t = warp_teacher<LIST == kTail, LIST == kTail>(s_list.l, a.K, a.inv_t);
-                const double rest = lse;
-                if (LIST == kTail) lse = log_add(rest, t.listed);
+                const Mass lse = LIST == kTail ? join_mass(rest, t.listed, a.inv_t) : rest;
                 double loss = 0.0;
                 for (int k = lane; k < a.K; k += 32)
                     if (s_list.l.used[k]) {
                         const double logq = (double)s_list.l.v[k] - (double)t.norm;
                         const double q = (double)expf((float)logq);
-                        const double z = (double)s_list.l.x[k] * a.inv_t;
-                        if (!(q <= 0.0)) loss += q * (logq - (z == -INFINITY ? z : z - lse));
+                        if (!(q <= 0.0)) loss += q * (logq - lse.below(s_list.l.x[k], a.inv_t));
                     }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
                 if (lane == 0) {
                     if (LIST == kTail) {
                         const double left = left_of(t, a.M);
-                        if (left > 0.0) loss += left * (log(left) - (rest == -INFINITY ? rest : rest - lse));
+                        if (left > 0.0)
+                            loss += left * (log(left) - (rest.log == -INFINITY
+                                                             ? rest.log
+                                                             : (rest.ref - lse.ref) * a.inv_t + rest.log - lse.log));
                     }
-                    if (s_list.l.bad || isnan(t.mass) || isnan(lse)) loss = NAN;
+                    if (s_list.l.bad || isnan(t.mass) || isnan(lse.log)) loss = NAN;
                     a.loss[row] = (float)loss;
-                    a.lse[row] = (float)lse;
-                    if (a.rest) a.rest[row] = (float)rest;
+                    a.lse[row] = limited(lse.value(a.inv_t));
+                    if (a.rest) a.rest[row] = limited(rest.value(a.inv_t));
                 }
             } else if (lane == 0) {
-                a.lse[row] = (float)lse;
-                // from the difference to ref, so that a large common offset costs nothing
+                a.lse[row] = limited(rest.value(a.inv_t));
                 const float x = Elem<T>::to_float(x_token);
                 if (a.logp)
                     a.logp[row] = token < 0        ? 0.0f
                                   : token >= a.M   ? NAN
-                                  : x == -INFINITY ? (isnan(lse) ? NAN : -INFINITY)
-                                                   : at_most_zero(((double)x - (double)w.ref) * a.inv_t - (double)logS);
+                                  : x == -INFINITY ? (isnan(logS) ? NAN : -INFINITY)
+                                                   : at_most_zero(rest.below(x, a.inv_t));
                 if (ENT) a.entropy[row] = w.S == 0.0f ? 0.0f : at_least_zero((double)logS - kLn2 * (double)(w.E / w.S));
                 s_ref = w.S == 0.0f ? 0.0 : (double)w.ref;
                 s_log = (double)logS;

@@ -768,3 +768,47 @@ def test_distill_rows_with_an_infinity_or_nan_are_nan(m, tail):
     for name in ("loss", "lse"):
         assert torch.isnan(out[name][:6]).all() and not torch.isnan(out[name][6:]).any(), name
     assert torch.isnan(out["dx"][:6]).all() and not torch.isnan(out["dx"][6:]).any()
+
+
+# ---- rows far from zero ------------------------------------------------------------------------------------
+def shifted(x):
+    """A row's logits below its largest, in 64 bits: log-probabilities, losses and gradients are the same, and no sum has
+    the size of the row's offset."""
+    x = x.double().cpu()
+    top = x.amax(1, keepdim=True)
+    return x - torch.where(torch.isinf(top), torch.zeros_like(top), top)
+
+
+def far_rows(m, dtype, seed):
+    """Rows of the type's lowest and highest values, of large common offsets, and masked with the lowest value."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = logits(8, m, dtype, seed)
+    x[0] = low                                        # a mask of the lowest value over the whole row
+    x[1] = low
+    x[1, 1::3] = -INF
+    x[2, ::2] = low                                   # ordinary: under such a mask
+    x[3] = high
+    x[4] = (x[4].float() * 8 + 3e4).to(dtype)
+    x[5] = (x[5].float() * 8 - 3e4).to(dtype)
+    x[6] = (x[6].float() + 700.0).to(dtype)
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m", [9, 1000, 33000])
+def test_distill_loss_of_rows_far_from_zero(m, dtype, tail):
+    k = 6
+    for t in (1.0, 0.5, 0.01):
+        x = far_rows(m, dtype, m)
+        n = x.shape[0]
+        index, values = teacher(n, m, k, m + 1)
+        out = run_distill(x.cuda(), index.cuda(), values.cuda(), t, tail, torch.ones(n).cuda())
+        near = shifted(x)
+        loss, _, _ = distill_rows(near, index, values, t, tail)
+        # q carries expf's error; log q - log p that of the row's sum, and a rounding of its own size
+        size = torch.where(torch.isfinite(near), near.abs(), torch.zeros_like(near)).gather(1, index).amax(1) / t
+        tol = room(x, t) + 8 * H * (40.0 + size) + 4 * H * loss.abs().nan_to_num(posinf=0.0)
+        close(out["loss"], loss.float(), tol)          # past the type's range: an infinity
+        assert torch.isfinite(out["lse"]).all()       # limited to the range of its type
