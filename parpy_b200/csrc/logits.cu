@@ -330,10 +330,12 @@ __device__ __forceinline__ float limited(double v) {
 
 // What one warp derives from a list: the teacher's normaliser and mass, the student's listed sum (natural logs).
 struct Teacher {
-    float norm;       // q_k = exp(v_k - norm)
+    float vref;       // log q_k = (v_k - vref) - norm: an offset common to the teacher's logits costs nothing
+    double norm;
     double mass;      // sum q (before `left`), in 64 bits: 1 - mass is next to a border
     Mass listed;      // log sum over the listed columns exp(z)
     int any;          // entries in use
+    __device__ double log_q(float v) const { return ((double)v - (double)vref) - norm; }
 };
 
 template <bool TAIL, bool STUDENT>
@@ -364,7 +366,8 @@ __device__ Teacher warp_teacher(const List &l, int K, double inv_t) {
     }
     Teacher t;
     t.any = n;
-    t.norm = TAIL || sv == 0.0 ? 0.0f : vref + (float)log(sv);    // no entry with mass: every q is exp(-inf) = 0
+    t.vref = TAIL ? 0.0f : vref;
+    t.norm = TAIL || sv == 0.0 ? 0.0 : log(sv);      // no entry with mass: every q is exp(-inf) = 0
     t.mass = !isfinite(sv) ? (double)NAN : TAIL ? sv : sv == 0.0 ? 0.0 : 1.0;
     // a sum that is not finite holds a NaN or +inf (finite columns are taken relative to their largest): the row is broken
     t.listed = {(double)xref, !STUDENT || sx == 0.0 ? -INFINITY : isfinite(sx) ? log(sx) : NAN};
@@ -705,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_stats(const RowAr
                 double loss = 0.0;
                 for (int k = lane; k < a.K; k += 32)
                     if (s_list.l.used[k]) {
-                        const double logq = (double)s_list.l.v[k] - (double)t.norm;
+                        const double logq = t.log_q(s_list.l.v[k]);
                         const double q = (double)expf((float)logq);
                         if (!(q <= 0.0)) loss += q * (logq - lse.below(s_list.l.x[k], a.inv_t));
                     }
@@ -893,11 +896,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
     } else {
         // the listed columns of this part's vectors, over what the pass wrote there (each column is listed once)
         __syncthreads();
-        const float norm = s_teacher.norm;
+        const Teacher teacher = s_teacher;
         for (int k = tid; k < a.K; k += THREADS)
             if (s_list.l.used[k] && ((s_list.l.col[k] + rv.mis) / VE) % total / THREADS == part) {
                 const double z = (double)s_list.l.x[k] * a.inv_t;
-                const float p = z == -INFINITY ? 0.0f : expf((float)(z - row_lse)), q = expf(s_list.l.v[k] - norm);
+                const float p = z == -INFINITY ? 0.0f : expf((float)(z - row_lse)), q = expf((float)teacher.log_q(s_list.l.v[k]));
                 dr[s_list.l.col[k]] =
                     Elem<T>::from_float(broken ? NAN : dead ? 0.0f : (float)(w * (W * (double)p - (double)q)));
             }

@@ -812,3 +812,20 @@ def test_distill_loss_of_rows_far_from_zero(m, dtype, tail):
         tol = room(x, t) + 8 * H * (40.0 + size) + 4 * H * loss.abs().nan_to_num(posinf=0.0)
         close(out["loss"], loss.float(), tol)          # past the type's range: an infinity
         assert torch.isfinite(out["lse"]).all()       # limited to the range of its type
+
+
+@gpu
+def test_teacher_values_far_from_zero():
+    # a teacher's logits with a common offset, or of the lowest value: the same probabilities as without
+    n, m, k = 5, 300, 9
+    x = logits(n, m, F32, 31)
+    index, values = teacher(n, m, k, 32)
+    values = (values * 64).round() / 64                      # offsets below leave them exact
+    far = values + torch.tensor([0.0, 512.0, -30000.0, 60000.0, 0.0])[:, None]
+    values[4], far[4] = 0.0, torch.finfo(F32).min
+    dloss = torch.ones(n).cuda()
+    out = run_distill(x.cuda(), index.cuda(), far.cuda(), 1.0, False, dloss)
+    check_distill(x.cuda(), index, values, 1.0, False, dloss, out)
+    # q only: the loss is free of the offset's size
+    loss, lse, _ = distill_rows(x, index, values, 1.0, False)
+    close(out["loss"], loss, room(x, 1.0) + 8 * H * (40.0 + lse.abs() + x.double().abs().amax(1)))
