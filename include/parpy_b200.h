@@ -358,6 +358,8 @@ int32_t parpy_b200_token_logprobs(const void *x, int32_t dtype, int64_t ldx, int
                                   int32_t wide_index, void *stream);
 /* Gradient with respect to x of sum(dlogp logp + dentropy entropy), from the lse and entropy that
  * the call above wrote: dx[N, M] (rows lddx apart) of x's element type, which may be x itself.
+ * lse far from 0 (|lse| > 64 in fp32, 1024 in 16 bits) does not bound the gradient's precision: such a row
+ * is summed again, unless its lse is another sum's (over more columns than these M), which is taken as it is.
  * dlogp, dentropy (and then tokens, entropy) may be NULL: no such term. */
 int32_t parpy_b200_token_logprobs_grad(const void *x, int32_t dtype, int64_t ldx, int64_t N, int64_t M,
                                        const void *tokens, int32_t wide_tokens, double temperature,

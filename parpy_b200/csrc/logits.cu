@@ -778,17 +778,86 @@ struct GradArgs {
     const float *lse, *entropy, *rest, *dlogp, *dentropy, *dloss;
 };
 
+// The sums of a gradient's row from the logits themselves, over vectors from, from + step, ... and all threads of the CTA; with
+// MASK the listed columns are left out. A vector of a list is found by a bit of its number (false hits cost a look).
+template <typename T, int THREADS, bool MASK>
+__device__ Sums row_sums(const Row<T> rv, const float c, const int from, const int step, const List *l,
+                                      const int K) {
+    constexpr int VE = Elem<T>::VE, NW = THREADS / 32, kMarks = 8192;
+    __shared__ Sums s_warp[NW];
+    __shared__ unsigned s_marks[MASK ? kMarks / 32 : 1];
+    const int tid = threadIdx.x, lane = tid & 31;
+    if constexpr (MASK) {
+        for (int i = tid; i < kMarks / 32; i += THREADS) s_marks[i] = 0;
+        __syncthreads();
+        for (int k = tid; k < K; k += THREADS)
+            if (l->used[k]) {
+                const int m = ((l->col[k] + rv.mis) / VE) % kMarks;
+                atomicOr(&s_marks[m >> 5], 1u << (m & 31));
+            }
+        __syncthreads();
+    }
+    Sums a{-INFINITY, 0.0f, 0.0f};
+    for (int v = from; v < rv.nvec; v += step) {
+        Vec r = rv.whole(v) ? ld_stream(rv.at(v)) : rv.edge(v);
+        if constexpr (MASK) {
+            const int m = v % kMarks;
+            if (s_marks[m >> 5] >> (m & 31) & 1u) {
+                T *e = reinterpret_cast<T *>(r.w);
+                const unsigned fill = Elem<T>::kFill;
+                for (int k = 0; k < K; ++k) {
+                    const int col = l->col[k] + rv.mis;
+                    if (!l->used[k] || col / VE != v) continue;
+#pragma unroll
+                    for (int i = 0; i < VE; ++i)
+                        if (i == col % VE) e[i] = *reinterpret_cast<const T *>(&fill);
+                }
+            }
+        }
+        const float vm = Elem<T>::vmax(r);
+        if (vm > a.ref) {
+            a.S = a.S == 0.0f ? 0.0f : a.S * pb::ex2_approx((a.ref - vm) * c);
+            a.ref = vm;
+        }
+        if (a.ref == -INFINITY) continue;
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+            float x0, x1;
+            Elem<T>::pair(r, i, x0, x1);
+            a.S += pb::ex2_approx((x0 - a.ref) * c) + pb::ex2_approx((x1 - a.ref) * c);
+        }
+    }
+    a = warp_join<false>(a, c);
+    if (lane == 0) s_warp[tid >> 5] = a;
+    __syncthreads();
+    return warp_join<false>(lane < NW ? s_warp[lane] : Sums{0.0f, 0.0f, 0.0f}, c);
+}
+
+// Whether `given`, in 32 bits, is this sum's rounding: half a step of it, and what two sums of a row may differ by. A sum over
+// more columns than the row's (a vocabulary in parts) is not, and is then taken as it was given.
+__device__ __forceinline__ bool same_sum(float given, const Mass &m, double inv_t) {
+    if (m.log == -INFINITY) return given == -INFINITY;
+    return fabs((double)limited(m.value(inv_t)) - (double)given) <= 0x1p-23 * fabs((double)given) + 0x1p-10;
+}
+
 // What bounds it: memory. One exp2, 10 instructions and 4 bytes a 16-bit logit; 4096 x 131072 bf16 in 346 us is 6.2 TB/s,
 // 95 % of the measured copy rate, 4096 x 65536 with the entropy's term in 176 us 93 %. A list's columns are written by a
 // second, short pass over what the first one wrote: to look for them within the first cost 1141 us.
 // grid.x = rows x parts; the vectors of a row are dealt round robin to the threads of its parts. Every element is
 // read and written by the same thread, so dx may be x itself (a list's logits are read before the first store only
 // within a CTA: in place needs parts = 1 there).
+//
+// lse (and rest) come in 32 bits: their rounding, up to 2^-24 |lse|, scales every probability of the row. Up to |lse| = 64 for
+// fp32 and 1024 for 16-bit gradients that is 2^-18 and 2^-14 (a value's own rounding: 2^-24; 2^-9 and 2^-12). Rows beyond,
+// whose logits share a large offset, lie under a mask of the type's lowest value, or meet a small temperature, are summed
+// again here in a pass of their own before the first store. `together`: the parts of a row are a cluster and share that
+// pass, because in place another part's stores would be under way.
 template <typename T, int THREADS, int LIST>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradArgs g, const int parts) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradArgs g, const int parts, const bool together) {
     constexpr int VE = Elem<T>::VE, U = 2;
     __shared__ ListSmem<THREADS, LIST == kNone ? kNone : kRenorm> s_list;
     __shared__ Teacher s_teacher;
+    __shared__ Sums s_part[LIST == kNone ? kMaxCluster : 1];
     const RowArgs &a = g.r;
     const int tid = threadIdx.x;
     const int part = blockIdx.x % parts;
@@ -803,13 +872,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
     // dx_j = e_j (al + be t_j), t_j = (x_j - ref) c, e_j = exp2(t_j), for every column but the token's
     // (gamma more) and the listed ones (written last). ref is lse (or rest) in units of x, as a high and a
     // low part, because its rounding would scale the whole row.
-    double base = (double)g.lse[row];
+    const float lse = g.lse[row];
+    double base = (double)lse;
     float al = 0.0f, be = 0.0f, gamma = 0.0f;
     long long token = -1;                     // its column, where this thread writes it
     float x_token = 0.0f;
-    double w = 0.0, W = 0.0, row_lse = base;
+    double w = 0.0, W = 0.0;
+    Mass row_lse{0.0, base};
     bool broken = false;
     const bool dead = base == -INFINITY;      // no finite logit in the row: no gradient
+    auto far_off = [&](float v) { return isfinite(v) && fabsf(v) > (sizeof(T) == 4 ? 64.0f : 1024.0f); };
+    float far_ref = 0.0f, far_log2 = 0.0f;    // of a row that is summed again
+    bool again = false;
     if constexpr (LIST == kNone) {
         if (a.tokens) token = load_index(a.tokens, row, a.wide);
         const double dl = g.dlogp && token >= 0 ? (double)g.dlogp[row] : 0.0;
@@ -824,31 +898,70 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
             x_token = Elem<T>::to_float(xr[token]);      // before it may be written over
         else
             token = -1;
+        if (far_off(lse)) {
+            Sums s = together ? row_sums<T, THREADS, false>(rv, c, me, total, nullptr, 0)
+                              : row_sums<T, THREADS, false>(rv, c, tid, THREADS, nullptr, 0);
+            if (together) {
+                cluster_arrive();             // every part runs before the first store into its shared memory
+                cluster_wait();
+                if (tid < parts) {
+                    const unsigned to = map_to_rank(smem_u32(&s_part[part]), tid);
+                    st_cluster_f32(to, s.ref);
+                    st_cluster_f32(to + 4, s.S);
+                }
+                cluster_arrive();
+                cluster_wait();
+                const int lane = tid & 31;
+                s = warp_join<false>(lane < parts ? Sums{s_part[lane].ref, s_part[lane].S, 0.0f} : Sums{0.0f, 0.0f, 0.0f}, c);
+            }
+            again = same_sum(lse, Mass{(double)s.ref, (double)logf(s.S)}, a.inv_t);
+            far_ref = s.ref;
+            far_log2 = log2f(s.S);
+        }
     } else {
         load_list(s_list.l, a, row, xr);
+        const bool far_row = far_off(lse) || (LIST == kTail && !dead && far_off(g.rest[row]));
         if (tid < 32) {
-            const Teacher t = warp_teacher<LIST == kTail, false>(s_list.l, a.K, a.inv_t);
+            const Teacher t = LIST == kTail && far_row ? warp_teacher<LIST == kTail, true>(s_list.l, a.K, a.inv_t)
+                                                       : warp_teacher<LIST == kTail, false>(s_list.l, a.K, a.inv_t);
             if (tid == 0) s_teacher = t;
         }
         __syncthreads();
         const Teacher t = s_teacher;
+        Mass rest{0.0, LIST == kTail ? (double)g.rest[row] : 0.0};
+        if (far_row) {
+            const Sums s = row_sums<T, THREADS, LIST == kTail>(rv, c, tid, THREADS, &s_list.l, a.K);
+            const Mass found{(double)s.ref, (double)logf(s.S)};
+            const Mass all = LIST == kTail ? join_mass(found, t.listed, a.inv_t) : found;
+            again = same_sum(lse, all, a.inv_t) && (LIST != kTail || same_sum(g.rest[row], found, a.inv_t));
+            if (again) {
+                row_lse = all;
+                rest = found;
+            }
+            far_ref = s.ref;
+            far_log2 = log2f(s.S);
+        }
         const double left = LIST == kTail ? left_of(t, a.M) : 0.0;
         w = (double)g.dloss[row] * a.inv_t;
         W = t.mass + left;
-        broken = s_list.l.bad || isnan(t.mass) || isnan(row_lse);
+        broken = s_list.l.bad || isnan(t.mass) || isnan(base);
         if (broken) {
             al = NAN;
         } else if (!dead && LIST == kTail) {
             // exp(z - rest) cannot overflow where it is used, however little the student has there
             base = (double)g.rest[row];
-            al = base == -INFINITY ? 0.0f : (float)(w * (W * exp(base - row_lse) - left));
+            al = rest.log == -INFINITY
+                     ? 0.0f
+                     : (float)(w * (W * exp((rest.ref - row_lse.ref) * a.inv_t + rest.log - row_lse.log) - left));
         } else if (!dead) {
             al = (float)(w * W);
         }
     }
     if (base == -INFINITY) base = 0.0;        // every x it meets is -inf: exp2(-inf) = 0
     base /= a.inv_t;
-    const float hi = (float)base, lo = (float)((base - (double)hi) * (double)c);
+    again = again && far_log2 != -INFINITY;
+    const float hi = again ? far_ref : (float)base;
+    const float lo = again ? far_log2 : (float)((base - (double)hi) * (double)c);
 
     auto slope = [&](float x) {
         const float t = fmaf(x - hi, c, -lo);
@@ -899,8 +1012,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
         const Teacher teacher = s_teacher;
         for (int k = tid; k < a.K; k += THREADS)
             if (s_list.l.used[k] && ((s_list.l.col[k] + rv.mis) / VE) % total / THREADS == part) {
-                const double z = (double)s_list.l.x[k] * a.inv_t;
-                const float p = z == -INFINITY ? 0.0f : expf((float)(z - row_lse)), q = expf((float)teacher.log_q(s_list.l.v[k]));
+                const float p = expf((float)row_lse.below(s_list.l.x[k], a.inv_t));
+                const float q = expf((float)teacher.log_q(s_list.l.v[k]));
                 dr[s_list.l.col[k]] =
                     Elem<T>::from_float(broken ? NAN : dead ? 0.0f : (float)(w * (W * (double)p - (double)q)));
             }
@@ -989,15 +1102,23 @@ int32_t launch_grad(const char *what, const GradArgs &g, cudaStream_t stream) {
     // large ones have less of a row's constants to make (4096 x 131072: 358 and 342 us)
     const bool big = bytes >= 192 * 1024, in_place = g.r.x == g.dx;
     const int threads = big ? 512 : 128;
+    // in place, a row's parts are a cluster, or one where there is a list
+    const int most = !in_place ? INT_MAX : LIST == kNone ? kMaxCluster : 1;
     int parts = 1;
-    while (!(LIST != kNone && in_place) && g.r.N * parts < 4LL * dev.sm_count &&
-           bytes / (2 * parts) >= (long long)threads * 16)
-        parts *= 2;
+    while (parts < most && g.r.N * parts < 4LL * dev.sm_count && bytes / (2 * parts) >= (long long)threads * 16) parts *= 2;
     PB_REQUIRE(g.r.N * parts <= INT_MAX, "%s: %lld rows are too many", what, g.r.N);
-    const unsigned grid = (unsigned)(g.r.N * parts);
-    if (big) row_grad<T, 512, LIST><<<grid, 512, 0, stream>>>(g, parts);
-    else row_grad<T, 128, LIST><<<grid, 128, 0, stream>>>(g, parts);
-    PB_CUDA(cudaGetLastError());
+    const bool together = in_place && parts > 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(g.r.N * parts));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = together ? 1 : 0;
+    auto kernel = big ? row_grad<T, 512, LIST> : row_grad<T, 128, LIST>;
+    PB_CUDA(cudaLaunchKernelEx(&cfg, kernel, g, parts, together));
     return PB_OK;
 }
 

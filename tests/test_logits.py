@@ -829,3 +829,98 @@ def test_teacher_values_far_from_zero():
     # q only: the loss is free of the offset's size
     loss, lse, _ = distill_rows(x, index, values, 1.0, False)
     close(out["loss"], loss, room(x, 1.0) + 8 * H * (40.0 + lse.abs() + x.double().abs().amax(1)))
+
+
+COARSE = {F32: 64.0 * H, BF16: 1024.0 * H, F16: 1024.0 * H}     # |lse| up to which its 32 bits serve the gradient
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m", [1, 9, 1000, 33000, 200003])
+def test_gradient_of_rows_far_from_zero(m, dtype):
+    # probabilities come from differences to the row's own sum, however large the offset or small the temperature:
+    # no term of the tolerance has the size of lse beyond the bound up to which its 32 bits are used
+    for t in (1.0, 0.5, 0.01, 1e-4):
+        x = far_rows(m, dtype, m + 1)
+        n = x.shape[0]
+        tokens = (torch.arange(n) * 7 % m).cuda()
+        xd = x.cuda()
+        out = run_logprobs(xd, tokens, 0, t)
+        d = define_logprobs(shifted(x), tokens, 0, t)
+        assert torch.isfinite(out["lse"]).all()
+        dl, de = torch.linspace(1, 2, n).cuda(), torch.linspace(0.5, -1, n).cuda()
+        size = d["p"] * (dl.cpu().abs()[:, None] + de.cpu().abs()[:, None] *
+                         (d["logps"].abs().clamp(max=200.0) + d["entropy"][:, None])) / t
+        rel = room(x, t) + COARSE[dtype] + 4 * H * d["logps"].abs().clamp(max=200.0)
+        off = d["p"] * de.cpu().abs()[:, None] * (room(x, t) * 20 + H * 400) / t
+        for bonus in (de, None):
+            want = define_logprobs_grad(d, tokens, dl, de if bonus is not None else torch.zeros(n), t)
+            tol = rounding(dtype, want) + size * rel + off + dl.cpu().abs()[:, None] * 2 * H / t
+            tol = tol + 210.0 * 2.0 ** -126 / t     # exp2 gives 0 below 2^-126, times |dlogp| + |dentropy| (|log p| + entropy)
+            dx = torch.full_like(xd, 7.0)
+            kernels.token_logprobs_grad(xd, tokens, n, m, t, out["lse"], out["entropy"], dl, bonus, dx, opts=opts())
+            close(dx, want, tol)
+            for rows in (slice(0, n), slice(0, 1)):      # in place, many rows and one
+                y = xd[rows].clone()
+                kernels.token_logprobs_grad(y, tokens[rows], y.shape[0], m, t, out["lse"][rows], out["entropy"][rows],
+                                            dl[rows], bonus[rows] if bonus is not None else None, y, opts=opts())
+                close(y, want[rows], tol[rows])
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [9, 1000, 33000])
+def test_distill_gradient_of_rows_far_from_zero(m, dtype, tail):
+    k = 6
+    for t in (1.0, 0.5, 0.01):
+        x = far_rows(m, dtype, m + 2)
+        x[7] = (x[7].float() - 90.0).to(dtype)
+        n = x.shape[0]
+        index, values = teacher(n, m, k, m + 3)
+        x[7, index[7]] = (x[7, index[7]].float() + 90.0).to(dtype)     # nearly nothing outside the list
+        dloss = torch.linspace(0.5, 1, n)
+        xd, idx, val = x.cuda(), index.cuda(), values.cuda()
+        out = run_distill(xd, idx, val, t, tail, dloss.cuda())
+        near = shifted(x)
+        d = define_distill(near, index, values, t, tail, dloss)
+        w = dloss.double()[:, None] / t
+        p = torch.exp(near / t - d["lse"][:, None])
+        rest = torch.where(torch.isfinite(d["rest"]), d["rest"], torch.full_like(d["rest"], INF))
+        pr = torch.exp(near / t - rest[:, None]).clamp(max=1.0)
+        rel = room(x, t) + 2 * COARSE[dtype] + 8 * H * (40.0 + torch.log(p).abs().clamp(max=200.0))
+        # exp2 gives 0 below 2^-126: an absolute error of p and pr, which w scales like every other
+        tol = rounding(dtype, d["dx"]) + w * ((p + pr * tail) * rel + 2.0 ** -125)
+        tol.scatter_add_(1, index, (w * 8 * H * 40.0).expand(n, k).contiguous())
+        close(out["dx"], d["dx"], tol)
+        y = xd.clone()
+        kernels.distill_topk_grad(y, idx, val, n, m, k, t, tail, out["lse"], out["rest"], dloss.cuda(), y, opts=opts())
+        close(y, d["dx"], tol)
+
+
+@gpu
+def test_gradient_takes_a_sum_over_more_columns_as_it_is():
+    # a vocabulary in two halves on two devices: each half's gradient from the sum over both, near zero and far from it
+    n, m = 6, 2002
+    x = logits(n, m, F32, 41)
+    x[3:] += 200.0
+    tokens = torch.arange(n)
+    out = run_logprobs(x.cuda(), tokens.cuda(), 0, 1.0)
+    dl = torch.ones(n).cuda()
+    none = torch.full((n,), -1)
+    d = define_logprobs(x, tokens, 0, 1.0)
+    want = define_logprobs_grad(d, tokens, dl, torch.zeros(n), 1.0)
+    for half, tok in ((slice(0, m // 2), tokens), (slice(m // 2, m), none)):
+        part, dx = x[:, half].contiguous().cuda(), torch.empty(n, m // 2, device="cuda")
+        scale = dl if tok is tokens else 3.0 * dl       # without a token there is no term
+        kernels.token_logprobs_grad(part, tok.cuda(), n, m // 2, 1.0, out["lse"], None, scale, None, dx, opts=opts())
+        expect = want[:, half] if tok is tokens else torch.zeros(n, m // 2)
+        close(dx, expect, d["p"][:, half] * (room(x, 1.0) + 250 * H + 80 * H) + 2.0 ** -22)
+    # the entropy's term needs no token
+    ones = torch.ones(n).cuda()
+    want = define_logprobs_grad(d, none, dl, ones, 1.0)
+    for half in (slice(0, m // 2), slice(m // 2, m)):
+        part, dx = x[:, half].contiguous().cuda(), torch.empty(n, m // 2, device="cuda")
+        kernels.token_logprobs_grad(part, None, n, m // 2, 1.0, out["lse"], out["entropy"], None, ones, dx, opts=opts())
+        size = d["p"][:, half] * (d["logps"][:, half].abs() + d["entropy"][:, None])
+        close(dx, want[:, half], size * (room(x, 1.0) + 330 * H) + d["p"][:, half] * (room(x, 1.0) * 20 + H * 400))
