@@ -396,7 +396,7 @@ int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, 
  * PARPY_B200_SCAN_TILE steps, which the gradient starts from (NULL where none is wanted).
  * lens[B] (NULL: all T; 64-bit where wide_lens is set; values outside [0, T] count as the nearest):
  * from lens[b] on the state is held, h, dg and dx are zero, and g, x, dh are not read.
- * Gates below -41.5 count as -41.5 (f = 2^-60). last may be h0; outputs must not overlap inputs
+ * Gates below -41.5 (fp32: -87) count as that (f = 2^-60; 1.6e-38). last may be h0; outputs must not overlap inputs
  * otherwise. No sum depends on the order in which threads arrive, nor on strides. */
 #define PARPY_B200_SCAN_TILE 128
 int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,

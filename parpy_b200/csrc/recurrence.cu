@@ -29,14 +29,15 @@ namespace {
 constexpr int kTile = PARPY_B200_SCAN_TILE;   // steps per tile, and per stored state
 constexpr int kMaxRanks = 8;
 constexpr int kStages = 3;                    // rounds of inputs in shared memory in the staged kernels
-constexpr float kCap = -41.5f;                // lowest gate value that is told apart (exact in all three types)
 
 // ---- four bytes of a row: the channels of one lane ------------------------------------------------------
+// kCap: the lowest gate value that is told apart, exact in its type (see gate()).
 template <typename T>
 struct Word;
 template <>
 struct Word<float> {
     static constexpr int CH = 1;
+    static constexpr float kCap = -87.0f;
     __device__ static void unpack(unsigned w, float (&v)[1]) { v[0] = __uint_as_float(w); }
     __device__ static unsigned cap(unsigned w) {        // max(v, kCap), NaN for NaN
         float r;
@@ -48,6 +49,7 @@ struct Word<float> {
 template <>
 struct Word<__nv_bfloat16> {
     static constexpr int CH = 2;
+    static constexpr float kCap = -41.5f;
     __device__ static void unpack(unsigned w, float (&v)[2]) {
         v[0] = __uint_as_float(w << 16);
         v[1] = __uint_as_float(w & 0xffff0000u);
@@ -64,6 +66,7 @@ struct Word<__nv_bfloat16> {
 template <>
 struct Word<__half> {
     static constexpr int CH = 2;
+    static constexpr float kCap = -41.5f;
     __device__ static void unpack(unsigned w, float (&v)[2]) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
         v[0] = f.x;
@@ -147,11 +150,11 @@ __device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
     return r;
 }
 
-// f = sigmoid(g) and 1 - f, each to its own relative precision: with e = exp(-g), f = 1 / (1 + e) and 1 - f = e f.
-// Two channels share one reciprocal, f_0 = d_1 / (d_0 d_1) with d = 1 + e (the special unit takes 16 a clock and SM, and
-// two of these for every value would be half of its time). g is capped from below at -41.5, where f = 2^-60 is nothing
-// beside 1 - f = 1, so that the product stays finite; a NaN gate, whose d the minimum leaves out of the product, stays in
-// its own channel.
+// f = sigmoid(g) and 1 - f, each to its own relative precision: with e = exp(-g), f = 1 / (1 + e) and 1 - f = e f. g is capped
+// from below so that e and f stay normal numbers: at -87 (f = 1.6e-38) where a channel has a reciprocal of its own. Two
+// 16-bit channels share one, f_0 = d_1 / (d_0 d_1) with d = 1 + e (the special unit takes 16 a clock and SM, and two of
+// these for every value would be half of its time): there at -41.5, where f = 2^-60 is nothing beside 1 - f = 1, so that the
+// product stays finite; a NaN gate, whose d the minimum leaves out of the product, stays in its own channel.
 __device__ __forceinline__ float reciprocal(float d) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
@@ -978,7 +981,7 @@ __global__ void __launch_bounds__(256) scan_step(const T *g, const T *x, const f
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
             const float v = (float)gv[k + j];
-            gk[j] = v < kCap ? kCap : v;
+            gk[j] = v < Word<T>::kCap ? Word<T>::kCap : v;
             xk[j] = (float)xv[k + j];
             sk[j] = sv[k + j];
         }

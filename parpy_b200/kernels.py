@@ -125,7 +125,7 @@ def gated_scan(g, x, h0, lens, B, T, D, h, last, carry):
     (None: T; clamped to [0, T]) on the state is held and h is zero. ``last`` [B,D] (or None) is the final state,
     ``carry`` [B,ceil(T/SCAN_TILE),D] (or None) the states that ``gated_scan_grad`` starts from; both float32,
     as h0; last may be h0. CUDA arrays g, x, h may be strided between sequences and between steps.
-    Gates below -41.5 count as -41.5."""
+    Gates below -41.5 (float32: -87) count as that."""
 
 
 @jit

@@ -531,3 +531,48 @@ def test_chunks_give_the_whole_sequence():
     r = room(s["g"], t)
     close(state, whole["last"], 2 * r * want["last_size"])
     close(h, whole["h"], 2 * (rounding(F32, want["h"]) + r * want["size"]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [70, 72])
+def test_gate_gradient_at_open_and_closed_gates(d, dtype):
+    b, t = 2, 3000
+    s = inputs(b, t, d, dtype, 15)
+    s["g"][:, :, ::3] = 12.0
+    s["g"][:, :, 1::3] = -100.0
+    s["g"][0, 100:140] = math.inf
+    s["g"][1, 50:60] = -math.inf
+    out = run(s, None)
+    floor = -87.0 if dtype == F32 else -41.5              # gates below count as this
+    want = define(s["g"].double().clamp(min=floor), s["x"], s["h0"], None, s["dh"], s["dlast"])
+    r = 2.0 ** -21 + 4 * H * t + 200 * 3 * H
+    both = want["r_size"] * (want["size"] + want["x"].abs() + s["h0"].abs().cpu().double()[:, None]) * want["keep"]
+    # behind a closed gate f (1 - f) is f, from the exponential of the whole gate value
+    close(out["dg"], want["dg"], rounding(dtype, want["dg"]) + 3 * r * both)
+    closed = (s["g"] <= -100.0).cpu()
+    near = torch.where(closed, want["dg"], torch.zeros_like(want["dg"]))
+    got = torch.where(closed, out["dg"].double().cpu(), torch.zeros_like(want["dg"]))
+    close(got, near, rounding(dtype, near) + 3 * r * both * torch.sigmoid(torch.tensor(floor, dtype=torch.float64)) +
+          2.0 ** -120)
+
+
+@gpu
+@pytest.mark.parametrize("d", [5, 64])
+def test_closed_gates_in_32_bits(d):
+    # an fp32 gate keeps its own value down to -87: f = exp(g) to a relative error, where 16-bit types stop at -41.5
+    b, t = 3, 4
+    s = inputs(b, t, d, F32, 17)
+    s["g"] = -torch.linspace(40.0, 86.0, b * t * d).reshape(b, t, d).cuda()
+    s["x"].zero_()
+    one = {k: (v[:, :1].contiguous() if v.dim() == 3 else v) for k, v in s.items()}
+    out = run(one, None, dlast=False)
+    f = torch.exp(one["g"].double().cpu())          # sigmoid and exp agree to exp(-40)
+    # the exponent's roundings of 86 log2(e), exp2, the sum with 1, the reciprocal and the products
+    rel = 86.0 * 1.5 * 2 * H + 2.0 ** -22 + 8 * H
+    h0, dh = s["h0"].double().cpu(), one["dh"].double().cpu()[:, 0]
+    close(out["last"], f[:, 0] * h0, rel * f[:, 0] * h0.abs() + 2.0 ** -148)
+    close(out["dh0"], f[:, 0] * dh, rel * f[:, 0] * dh.abs() + 2.0 ** -148)
+    h, last = torch.empty(b, d, device="cuda"), torch.empty(b, d, device="cuda")
+    kernels.gated_step(one["g"][:, 0], one["x"][:, 0], s["h0"], b, d, h, last, opts=opts())
+    assert torch.equal(last, out["last"])
