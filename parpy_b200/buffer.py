@@ -42,10 +42,17 @@ def _extract_array_interface(a, allow_cuda=False, pitched=False):
             raise ValueError("Buffers must only operate on contiguous memory")
         return tuple(a.shape), DataType("<V2"), a.data_ptr()
     if hasattr(a, "__array_interface__"):
-        return _check_array_interface(a.__array_interface__)
+        return _check_host_interface(a.__array_interface__)
     if hasattr(a, "__array__"):
-        return _check_array_interface(a.__array__().__array_interface__)
+        return _check_host_interface(a.__array__().__array_interface__)
     raise ValueError("Failed to extract array interface")
+
+
+def _check_host_interface(intf):
+    shape, dtype, data = _check_array_interface(intf)
+    if dtype.sz is ElemSize.BF16:       # host arrays are read through NumPy, which has no such type
+        raise RuntimeError(f"Unknown type identifier {dtype.sz.value}")
+    return shape, dtype, data
 
 
 def _is_host_bf16(a):

@@ -93,6 +93,8 @@ class DataType:
             self.sz = ElemSize(typestr[1:])
         except ValueError:
             raise RuntimeError(f"Unknown type identifier {typestr[1:]}")
+        if self.sz is ElemSize.BF16 and typestr[0] == "|":       # NumPy's two-byte void type, no number
+            raise RuntimeError(f"Unknown type identifier {typestr[1:]}")
         self.typestr = typestr
 
     @staticmethod

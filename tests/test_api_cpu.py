@@ -233,3 +233,21 @@ def test_kernels_read_only_prefixed_environment_names():
         for argument in found:
             quoted = re.findall(r'"([^"]*)"', argument)
             assert quoted and all(name.startswith("PARPY_B200_") for name in quoted), (file, argument)
+
+
+def test_two_byte_void_arrays_are_not_bfloat16():
+    # NumPy's own two-byte void type ('|V2') is no number; a bfloat16 array says '<V2'
+    for a in (np.zeros(3, "V2"), np.zeros(3, [("a", "i1"), ("b", "i1")])):
+        with pytest.raises(RuntimeError, match="Unknown type identifier V2"):
+            buffer.from_array(a, None)
+        with pytest.raises(RuntimeError, match="Unknown type identifier V2"):
+            buffer._extract_array_interface(a)
+    with pytest.raises(RuntimeError, match="Unknown type identifier V2"):
+        DataType("|V2")
+
+    class Little:           # a host array that says bfloat16 without being a tensor: nothing here reads it
+        __array_interface__ = {"shape": (3,), "typestr": "<V2", "data": (np.zeros(3, np.int16).ctypes.data, False),
+                               "strides": None, "version": 3}
+    with pytest.raises(RuntimeError, match="Unknown type identifier V2"):
+        buffer._extract_array_interface(Little())
+    assert DataType("<V2").sz is parpy.types.BF16 and DataType.from_elem_size(parpy.types.BF16) == DataType("<V2")
