@@ -120,19 +120,22 @@ class Buffer:
             self.refcount = refcount
             self.refcount[0] += 1
 
+    def _item(self):
+        return self.numpy().item()
+
     def __float__(self):
         if len(self.shape) == 0:
-            return float(self.numpy().item())
+            return float(self._item())
         raise ValueError(f"Cannot convert buffer of shape {self.shape} to float")
 
     def __int__(self):
         if len(self.shape) == 0:
-            return int(self.numpy().item())
+            return int(self._item())
         raise ValueError(f"Cannot convert buffer of shape {self.shape} to int")
 
     def __bool__(self):
         if len(self.shape) == 0:
-            return bool(self.numpy().item())
+            return bool(self._item())
         raise ValueError(f"Cannot convert buffer of shape {self.shape} to bool")
 
     def __index__(self):
@@ -204,7 +207,11 @@ class CudaBuffer(Buffer):
     def sync(self):
         sync(self.backend)
 
+    def _item(self):
+        return self.buf.item()
+
     def numpy(self):
+        self.dtype.to_numpy()       # refuses bfloat16 by name
         return np.asarray(self.buf.cpu())
 
     def torch(self):
@@ -253,6 +260,7 @@ class DummyBuffer(Buffer):
         return self.buf
 
     def numpy(self):
+        self.dtype.to_numpy()       # refuses bfloat16 by name
         return np.asarray(self)
 
 

@@ -251,3 +251,19 @@ def test_two_byte_void_arrays_are_not_bfloat16():
     with pytest.raises(RuntimeError, match="Unknown type identifier V2"):
         buffer._extract_array_interface(Little())
     assert DataType("<V2").sz is parpy.types.BF16 and DataType.from_elem_size(parpy.types.BF16) == DataType("<V2")
+
+
+def test_bfloat16_buffers_give_numbers_and_refuse_numpy():
+    import torch
+    one = torch.tensor(1.5, dtype=torch.bfloat16)
+    b = buffer.CudaBuffer(one, (), parpy.types.BF16)
+    assert float(b) == 1.5 and int(b) == 1 and bool(b) is True and ops.scalar(b, "b") == 1.5
+    with pytest.raises(ValueError, match="as index"):
+        b.__index__()
+    with pytest.raises(RuntimeError, match="NumPy has no bfloat16 type"):
+        b.numpy()
+    host = torch.zeros(3, dtype=torch.bfloat16)
+    dummy = buffer.from_array(host, None)
+    assert dummy.shape == (3,) and dummy.dtype.sz is parpy.types.BF16
+    with pytest.raises(RuntimeError, match="NumPy has no bfloat16 type"):
+        dummy.numpy()
