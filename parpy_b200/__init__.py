@@ -53,8 +53,8 @@ def _check_kwargs(kwargs, fun_name):
 
 def _role_of(spec, opts, name, key=None):
     r = spec.roles.get(name, "in")
-    if key is not None:
-        r = r.get(key, "in") if isinstance(r, dict) else r
+    if isinstance(r, dict):
+        r = r.get(key, "in")        # no key: an array where a dictionary belongs, which the operator refuses
     if callable(r):
         r = r(opts)
     return r
@@ -112,6 +112,8 @@ def _as_they_are(spec, args, kwargs):
     if (device, _native.LIB_PATH) not in backend._usable:
         return False
     tensors, types, strided = torch.Tensor, _torch_dtypes(), torch.strided
+    if True in spec.keyed:
+        return False            # dictionaries, or the refusal of something else in their place
     for arg, pitched in zip(args, spec.pitched):
         kind = type(arg)
         if kind is tensors:

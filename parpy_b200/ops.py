@@ -33,6 +33,7 @@ class OpSpec:
         self.adapter = adapter
         self.doc = doc
         self.pitched = tuple(str(roles.get(p)).endswith("_rows") for p in self.params)
+        self.keyed = tuple(isinstance(roles.get(p), dict) for p in self.params)
 
 
 REGISTRY = {}   # name -> [OpSpec]

@@ -267,3 +267,22 @@ def test_bfloat16_buffers_give_numbers_and_refuse_numpy():
     assert dummy.shape == (3,) and dummy.dtype.sz is parpy.types.BF16
     with pytest.raises(RuntimeError, match="NumPy has no bfloat16 type"):
         dummy.numpy()
+
+
+def test_an_array_in_the_place_of_a_dictionary_goes_the_long_way():
+    # the parameter's roles are by key there; an array in its place is staged as an input and refused by the operator
+    spec = ops.REGISTRY["spmv_row"][0]
+    assert parpy._role_of(spec, parpy.par({}), "A") == "in" and parpy._role_of(spec, parpy.par({}), "A", "cols") == "in"
+    assert parpy._role_of(spec, parpy.par({}), "x") == "in" and parpy._role_of(spec, parpy.par({}), "y") == "inout"
+    assert spec.keyed == (True, False, False)
+
+
+@pytest.mark.gpu
+def test_an_array_in_the_place_of_a_dictionary_is_refused():
+    import torch
+    from parpy_b200 import kernels
+    v = torch.zeros(4, device="cuda")
+    for a in (v, np.zeros(4, np.float32), buffer.from_array(np.zeros(4, np.float32))):
+        for other in (v, np.zeros(4, np.float32)):
+            with pytest.raises(TypeError, match="not subscriptable"):
+                kernels.spmv_row(a, other, other, opts=parpy.par({}))
