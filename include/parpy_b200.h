@@ -341,8 +341,9 @@ int32_t parpy_b200_viterbi_wait_probe(int32_t polls, void *stream);
  * apart (any pitch >= M and any alignment of the element type); z = x / temperature, with
  * temperature in [1e-4, 1e4]. A logit of -inf is a column that a mask took out. Sums are kept in
  * 32 bits, each output is rounded once. A row that holds a NaN or +inf gets NaN outputs
- * (top_index -1); a row without a finite logit has lse -inf, logp -inf and a zero
- * gradient. lse and rest of a row with one are finite: they stop at the range of a float. Token and column numbers are 64-bit where the wide_ flag is set, else 32-bit. */
+ * (top_index -1; rest is NaN where such a column is not listed); a row without a finite logit has lse
+ * -inf, logp -inf and a zero gradient. lse and rest of a row with one are finite: they stop at the
+ * range of a float. Token and column numbers are 64-bit where the wide_ flag is set, else 32-bit. */
 #define PARPY_B200_F32 0
 #define PARPY_B200_BF16 1
 #define PARPY_B200_F16 2
@@ -391,13 +392,16 @@ int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, 
  * No counterpart in the reference; its nearest function is the recurrence over observation
  * sequences of benchmarks/forward.py:94-187. f = sigmoid(g), h_t = f_t h_{t-1} + (1 - f_t) x_t for
  * every channel of g, x [B, T, D] (element type `dtype`: PARPY_B200_F32, _BF16, _F16). _sb and _st are the
- * elements between sequences and between steps of an array; channels are contiguous. States are kept in 32 bits: h0[B, D] (NULL: zeros), last[B, D] (NULL: not written), and
+ * elements between sequences and between steps of an array; channels are contiguous. States are kept
+ * in 32 bits: h0[B, D] (NULL: zeros), last[B, D] (NULL: not written), and
  * carry[B, ceil(T / PARPY_B200_SCAN_TILE), D], the state that enters each run of
  * PARPY_B200_SCAN_TILE steps, which the gradient starts from (NULL where none is wanted).
  * lens[B] (NULL: all T; 64-bit where wide_lens is set; values outside [0, T] count as the nearest):
  * from lens[b] on the state is held, h, dg and dx are zero, and g, x, dh are not read.
- * Gates below -41.5 (fp32: -87) count as that (f = 2^-60; 1.6e-38). last may be h0; outputs must not overlap inputs
- * otherwise. No sum depends on the order in which threads arrive, nor on strides. */
+ * Gates below -41.5 (fp32: -87) count as that (f = 2^-60; 1.6e-38). An infinity or NaN in a state, input
+ * or gate makes every later step of its channel infinite or NaN (not always the one that the steps
+ * one by one would give) and reaches no other channel. last may be h0; outputs must not overlap
+ * inputs otherwise. No sum depends on the order in which threads arrive, nor on strides. */
 #define PARPY_B200_SCAN_TILE 128
 int32_t parpy_b200_gated_scan(int32_t dtype, int64_t B, int64_t T, int64_t D, const void *g, int64_t g_sb,
                               int64_t g_st, const void *x, int64_t x_sb, int64_t x_st, const float *h0,

@@ -14,6 +14,10 @@
 //
 // and rebuilds the states in 32 bits from the one that the forward kernel stored at the start of every tile (1/128 of
 // their bytes) instead of reading back h, which has been rounded to the output type.
+//
+// An infinite or NaN state, input or gate reaches every later step of its channel (and every earlier one's gradient) as an
+// infinity or NaN, and no other channel. Which of the two is not the stepwise definition's: a run's A that has underflowed to
+// 0 makes NaN of an infinity.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -939,8 +943,9 @@ __global__ void __launch_bounds__(W * 32) scan_backward_staged(const ScanArgs a,
     if (a.dh0 && rank == 0 && warp < CH && mine < n) a.dh0[(long long)b * a.D + c0 + mine] = back;
 }
 
-// ---- one token for every row (bounded by memory: 2048 x 8192 bf16 in 38 us, 93 % of the measured copy rate): 8 channels per thread where the rows allow 16-byte access, else 2 ----------------
-// (2, because a pair of 16-bit channels shares its reciprocal: the step then has the scan's bits.)
+// ---- one token for every row (bounded by memory: 2048 x 8192 bf16 in 38 us, 93 % of the measured copy rate) --------
+// 8 channels per thread where the rows allow 16-byte access, else 2 (2, because a pair of 16-bit channels shares its
+// reciprocal: the step then has the scan's bits).
 template <typename T, int VN>
 __global__ void __launch_bounds__(256) scan_step(const T *g, const T *x, const float *state, T *h, float *last,
                                                  long long N, int D, long long ldg, long long ldx, long long ldh) {

@@ -8,8 +8,10 @@ of a long vector.
 
 Beside them stand operators of language models on the same kinds of data: on rows of
 vocabulary logits ``token_logprobs`` and ``distill_topk`` with their gradients; over
-padded sequences the recurrence ``gated_scan`` with its gradient and, for decoding, ``gated_step``. They take float32, bfloat16 and float16 and, for CUDA arrays, rows that lie apart (a slice of a wider
-matrix); arguments that may be ``None`` are named in their docstrings."""
+padded sequences the recurrence ``gated_scan`` with its gradient and, for decoding,
+``gated_step``. They take float32, bfloat16 and float16 and, for CUDA arrays, rows that
+lie apart (a slice of a wider matrix); arguments that may be ``None`` are named in their
+docstrings, and outputs overlap inputs only where those say so."""
 from . import jit
 from ._native import SCAN_TILE
 
@@ -91,14 +93,17 @@ def token_logprobs(x, tokens, N, M, K, temperature, logp, lse, entropy, top_logp
     their log-probabilities top_logp[N,K] and numbers top_index[N,K]. A logit of -inf is a column that a
     mask took out; a row of nothing else has lse and logp -inf and entropy 0; a row with a
     NaN or +inf gets NaN (top_index -1). ``tokens`` with ``logp``, ``entropy``, and for K = 0 ``top_logp``
-    and ``top_index`` may be None. lse (and entropy) are what the gradient needs."""
+    and ``top_index`` may be None. lse (and entropy) are what the gradient needs; lse stops at the range
+    of float32."""
 
 
 @jit
 def token_logprobs_grad(x, tokens, N, M, temperature, lse, entropy, dlogp, dentropy, dx):
     """dx[N,M] = gradient of sum(dlogp * logp + dentropy * entropy) with respect to x, in x's
-    type; dx may be x, and must not overlap it otherwise. ``dlogp`` (then ``tokens``) and ``dentropy`` (then ``entropy``) may be None.
-    The alternatives are reported, not differentiated. A row without a finite logit gets zeros."""
+    type; dx may be x, and must not overlap it otherwise. ``dlogp`` (then ``tokens``) and ``dentropy``
+    (then ``entropy``) may be None. ``lse`` and ``entropy`` are what ``token_logprobs`` wrote for the same
+    arguments. The alternatives are reported, not differentiated. A row without a finite logit gets zeros.
+    Rows with abs(lse) above 64 (16-bit types: 1024) are summed again, which costs them a second pass."""
 
 
 @jit
@@ -114,8 +119,10 @@ def distill_topk(x, index, values, N, M, K, temperature, tail, loss, lse, rest):
 
 @jit
 def distill_topk_grad(x, index, values, N, M, K, temperature, tail, lse, rest, dloss, dx):
-    """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x, and must
-    not overlap it otherwise. ``lse`` and ``rest`` are what ``distill_topk`` wrote for the same arguments."""
+    """dx[N,M] = gradient of sum(dloss * loss) with respect to x, in x's type; dx may be x (few long rows
+    take longer then: one CTA a row), and must not overlap it otherwise. ``lse`` and ``rest`` are what
+    ``distill_topk`` wrote for the same arguments; rows where one of them is above 64 (16-bit types: 1024)
+    in size are summed again."""
 
 
 @jit
@@ -124,8 +131,8 @@ def gated_scan(g, x, h0, lens, B, T, D, h, last, carry):
     from the state h0[B,D] (None: zeros), in 32 bits, h rounded once to the type of x. From lens[b]
     (None: T; clamped to [0, T]) on the state is held and h is zero. ``last`` [B,D] (or None) is the final state,
     ``carry`` [B,ceil(T/SCAN_TILE),D] (or None) the states that ``gated_scan_grad`` starts from; both float32,
-    as h0; last may be h0. CUDA arrays g, x, h may be strided between sequences and between steps.
-    Gates below -41.5 (float32: -87) count as that."""
+    as h0; last may be h0. CUDA arrays g, x, h may be strided between sequences and between steps. An infinity or
+    NaN makes the later steps of its channel infinite or NaN. Gates below -41.5 (float32: -87) count as that."""
 
 
 @jit

@@ -576,3 +576,24 @@ def test_closed_gates_in_32_bits(d):
     h, last = torch.empty(b, d, device="cuda"), torch.empty(b, d, device="cuda")
     kernels.gated_step(one["g"][:, 0], one["x"][:, 0], s["h0"], b, d, h, last, opts=opts())
     assert torch.equal(last, out["last"])
+
+
+@gpu
+def test_an_infinite_input_stays_in_its_channel():
+    # from its step on an infinity leaves infinities or NaN (a product of gates that has underflowed, times it) in its
+    # channel, and nothing anywhere else
+    b, t, d = 2, 2000, 72
+    for dtype in (F32, BF16):
+        s = inputs(b, t, d, dtype, 16)
+        clean = run(s, None)
+        s["x"][0, 700, 6] = math.inf
+        s["h0"][1, 9] = -math.inf
+        dirty = run(s, None)
+        hit = torch.zeros(b, d, dtype=torch.bool, device="cuda")
+        hit[0, 6] = hit[1, 9] = True
+        for name in ("h", "dx"):
+            keep = (~hit)[:, None].expand(b, t, d)
+            assert torch.equal(clean[name][keep], dirty[name][keep])
+        assert torch.equal(clean["last"][~hit], dirty["last"][~hit]) and not torch.isfinite(dirty["last"][hit]).any()
+        assert torch.equal(clean["h"][0, :700, 6], dirty["h"][0, :700, 6])
+        assert not torch.isfinite(dirty["h"][0, 700:, 6]).any() and not torch.isfinite(dirty["h"][1, :, 9]).any()
