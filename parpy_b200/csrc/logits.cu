@@ -419,7 +419,10 @@ __device__ __forceinline__ void st_cluster_u64(unsigned addr, u64 v) {
 // all above half; the rest is a row's end, where its CTA loads nothing. Measured: 4096 x 131072 bf16 without entropy
 // 194 us (84 % of the copy rate), 4096 x 65536 with entropy 117 us (70 %), 4096 x 131072 with entropy and 20 alternatives
 // 256 us (64 %). 128 threads a row keep more rows apart in their phases than 256 (distillation 194 against 211 us); the
-// selection's end and a tail's list are shared by 256 (257 against 300 us; 45 against 53 us). Held in registers two
+// selection's end and a tail's list are shared by 256 (257 against 300 us; 45 against 53 us). The second look of a
+// selection costs 16 % of the row's bytes again (1184 rows: 360 MB read for 310), in pieces of 32 bytes of the few threads
+// that pass the bound; a row's end keeps one vector a thread in flight. 64 registers leave 28 to 76 bytes of spills in
+// most instances with entropy or alternatives (one warp a row with both: 276), none without. Held in registers two
 // stages deep: loads that pass through shared memory (cp.async, four stages) cost 218 instead of 209 us, in 16-byte
 // pieces of a lane's own vector 322 us; scalar arithmetic instead of packed pairs 132 instead of 120 us.
 template <typename T, int THREADS, bool ENT, bool TOP, int LIST>
@@ -840,8 +843,8 @@ __device__ __forceinline__ bool same_sum(float given, const Mass &m, double inv_
     return fabs((double)limited(m.value(inv_t)) - (double)given) <= 0x1p-23 * fabs((double)given) + 0x1p-10;
 }
 
-// What bounds it: memory. One exp2, 10 instructions and 4 bytes a 16-bit logit; 4096 x 131072 bf16 in 346 us is 6.2 TB/s,
-// 95 % of the measured copy rate, 4096 x 65536 with the entropy's term in 176 us 93 %. A list's columns are written by a
+// What bounds it: memory. One exp2, 10 instructions and 4 bytes a 16-bit logit; 4096 x 131072 bf16 with a list in 350 us is
+// 6.1 TB/s, 93 % of the measured copy rate, 4096 x 65536 with the entropy's term in 178 us 92 %. A list's columns are written by a
 // second, short pass over what the first one wrote: to look for them within the first cost 1141 us.
 // grid.x = rows x parts; the vectors of a row are dealt round robin to the threads of its parts. Every element is
 // read and written by the same thread, so dx may be x itself (a list's logits are read before the first store only
@@ -912,7 +915,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) row_grad(const GradAr
                 cluster_arrive();
                 cluster_wait();
                 const int lane = tid & 31;
-                s = warp_join<false>(lane < parts ? Sums{s_part[lane].ref, s_part[lane].S, 0.0f} : Sums{0.0f, 0.0f, 0.0f}, c);
+                s = lane < parts ? Sums{s_part[lane].ref, s_part[lane].S, 0.0f} : Sums{0.0f, 0.0f, 0.0f};
+                s = warp_join<false>(s, c);
             }
             again = same_sum(lse, Mass{(double)s.ref, (double)logf(s.S)}, a.inv_t);
             far_ref = s.ref;
@@ -1132,13 +1136,11 @@ int32_t check_gradient(const char *what, const void *x, int32_t dtype, int64_t l
     return PB_OK;
 }
 
-int32_t check_list(const char *what, const void *index, const void *values, int32_t value_dtype, int64_t K,
-                   int64_t M) {
+int32_t check_list(const char *what, const void *index, const void *values, int32_t value_dtype, int64_t K) {
     PB_REQUIRE(index && values, "%s: null pointer", what);
     PB_REQUIRE(K >= 1 && K <= kListMax, "%s: K=%lld is outside [1, %d]", what, (long long)K, kListMax);
     PB_REQUIRE(value_dtype == PARPY_B200_F32 || value_dtype == PARPY_B200_BF16 || value_dtype == PARPY_B200_F16,
                "%s: unknown element type %d", what, value_dtype);
-    (void)M;
     return PB_OK;
 }
 
@@ -1210,7 +1212,7 @@ int32_t parpy_b200_distill_topk(const void *x, int32_t dtype, int64_t ldx, int64
                                 double temperature, int32_t tail, float *loss, float *lse, float *rest, void *stream) {
     int32_t rc = check_rows("distill_topk", x, dtype, ldx, N, M, temperature);
     if (rc || N == 0) return rc;
-    rc = check_list("distill_topk", index, values, value_dtype, K, M);
+    rc = check_list("distill_topk", index, values, value_dtype, K);
     if (rc) return rc;
     PB_REQUIRE(loss && lse && (!tail || rest), "distill_topk: null pointer");
     RowArgs a = {};
@@ -1239,7 +1241,7 @@ int32_t parpy_b200_distill_topk_grad(const void *x, int32_t dtype, int64_t ldx, 
     int32_t rc = check_rows("distill_topk_grad", x, dtype, ldx, N, M, temperature);
     if (!rc) rc = check_gradient("distill_topk_grad", x, dtype, ldx, N, M, dx, lddx);
     if (rc || N == 0) return rc;
-    rc = check_list("distill_topk_grad", index, values, value_dtype, K, M);
+    rc = check_list("distill_topk_grad", index, values, value_dtype, K);
     if (rc) return rc;
     PB_REQUIRE(lse && dloss && (!tail || rest), "distill_topk_grad: null pointer");
     GradArgs g = {};

@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(W * 32) scan_backward(const ScanArgs a, const 
 // in place by the results, and written back 16 bytes a lane during the next round's exchange.
 //
 // Measured (bf16): 1 x 65536 x 2048 in 195 us (4.1 TB/s, 63 % of the measured copy rate), 16 x 1000..4000 x 2048 forward in
-// 117 us (84 %) and backward in 223 us (66 %). What bounds them: a round is a chain of barriers (fold, exchange,
+// 110 us (78 %) and backward in 225 us (66 %); fp32, 16 x 1000..4000 x 1024, in 105 us (82 %) and 180 us (82 %). What bounds them: a round is a chain of barriers (fold, exchange,
 // step), and the two CTAs of an SM (one, backward) do not fill each other's waits; without the exchange between
 // the cluster's CTAs the long sequence would take 164 us, without the gates 176 us, without both 143 us. Loading and
 // storing 4 bytes a lane and step straight from global memory spends two thirds of the instructions on addresses (270 us,
