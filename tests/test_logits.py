@@ -924,3 +924,58 @@ def test_gradient_takes_a_sum_over_more_columns_as_it_is():
         kernels.token_logprobs_grad(part, None, n, m // 2, 1.0, out["lse"], out["entropy"], None, ones, dx, opts=opts())
         size = d["p"][:, half] * (d["logps"][:, half].abs() + d["entropy"][:, None])
         close(dx, want[:, half], size * (room(x, 1.0) + 330 * H) + d["p"][:, half] * (room(x, 1.0) * 20 + H * 400))
+
+
+@gpu
+def test_gradients_in_place_captured_and_at_once():
+    # few rows in place (a row's CTAs share a sum where it is far from zero) and with a list, each in a graph of its own,
+    # both replayed at once on two streams over new logits
+    n, m, k = 3, 70001, 9
+    tokens, dl = torch.arange(n, device="cuda") * 5, torch.ones(n, device="cuda")
+    index, values = (v.cuda() for v in teacher(n, m, k, 51))
+    for dtype in (F32, BF16):
+        source = logits(n, m, dtype, 50).cuda()
+        y, z = torch.empty_like(source), torch.empty_like(source)
+        logp, lse, entropy = (torch.empty(n, device="cuda") for _ in range(3))
+        loss, lse2, rest = (torch.empty(n, device="cuda") for _ in range(3))
+
+        def one(y=y):
+            o = opts()
+            y.copy_(source)
+            kernels.token_logprobs(y, tokens, n, m, 0, 0.5, logp, lse, entropy, None, None, opts=o)
+            kernels.token_logprobs_grad(y, tokens, n, m, 0.5, lse, entropy, dl, dl, y, opts=o)
+
+        def other(z=z):
+            o = opts()
+            z.copy_(source)
+            kernels.distill_topk(z, index, values, n, m, k, 0.5, True, loss, lse2, rest, opts=o)
+            kernels.distill_topk_grad(z, index, values, n, m, k, 0.5, True, lse2, rest, dl, z, opts=o)
+        graphs = []
+        for call in (one, other):
+            call()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                call()
+            graphs.append(graph)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for offset in (0.0, 2000.0, -300.0):
+            source.copy_(logits(n, m, dtype, 52) + torch.tensor([offset, 0.0, -offset])[:, None].to(dtype))
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for graph, stream in zip(graphs, streams):
+                    with torch.cuda.stream(stream):
+                        graph.replay()
+            torch.cuda.synchronize()
+            got = y.clone(), z.clone()
+            out = run_logprobs(source, tokens, 0, 0.5)
+            apart = torch.empty_like(source)
+            kernels.token_logprobs_grad(source, tokens, n, m, 0.5, out["lse"], out["entropy"], dl, dl, apart, opts=opts())
+            d = define_logprobs(shifted(source), tokens, 0, 0.5)
+            want = define_logprobs_grad(d, tokens, dl, dl, 0.5)
+            size = d["p"] * (1 + d["logps"].abs().clamp(max=200.0) + d["entropy"][:, None]) / 0.5
+            rel = room(source, 0.5) + COARSE[dtype] + 4 * H * d["logps"].abs().clamp(max=200.0)
+            tol = rounding(dtype, want) + size * rel + d["p"] * (room(source, 0.5) * 20 + H * 400) / 0.5 + 4 * H + 2.0 ** -117
+            close(apart, want, tol)
+            close(got[0], want, tol)
+            same = run_distill(source, index, values, 0.5, True, dl)
+            assert torch.equal(got[1], same["dx"]) and torch.equal(loss, same["loss"])
